@@ -242,6 +242,11 @@ def prepare(case, seed):
 
 
 # ------------------------------------------------------------------------------------------------- the definition in 64 bits
+def _two_to(e):
+    """2.0 ** e in float64 from its bits (the device's pow is off by an ulp for some whole e, which would move ties)."""
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
 def _round_exact(x):
     """Values that MXFP4 holds for x [R, K], straight from the definition: the nearest member of the scaled grid, the even code of two
     that are equally near."""
@@ -252,7 +257,7 @@ def _round_exact(x):
     for r in range(0, R, 4096):
         b = x[r:r + 4096].double().reshape(-1, BLOCK)
         top = b.abs().max(dim=1, keepdim=True).values
-        unit = torch.pow(2.0, torch.floor(torch.log2(top)) - 2).clamp(min=2.0 ** -127)
+        unit = _two_to((torch.frexp(top)[1] - 3).clamp(min=-127))           # floor(log2 top) - 2
         a = (b / unit).abs()
         code = torch.zeros_like(a, dtype=torch.int64)
         for i, mid in enumerate(mids.tolist()):
@@ -266,7 +271,7 @@ def _values_exact(codes, scales):
     c = torch.stack((lo, hi), -1).flatten(-2)
     grid = torch.tensor(GRID, dtype=torch.float64, device=codes.device)
     v = grid[c & 7] * (1.0 - 2.0 * (c >> 3).double())
-    return v * torch.pow(2.0, scales.double() - 127).repeat_interleave(BLOCK, -1)
+    return v * _two_to(scales.int() - 127).repeat_interleave(BLOCK, -1)
 
 
 def exact(case, seed):
