@@ -1,0 +1,282 @@
+// KV cache held in MXFP4 (format: mxfp4.h) and single-token attention over it.
+//
+// Layout, per K and V: codes [B, Hkv, max_len, dh / 2], scales [B, Hkv, max_len, dh / 32] — the rows of one head are contiguous (a
+// 128-wide key is 64 + 4 bytes), blocks run along the head dimension, so a token is appended without touching its neighbours.
+//
+// Attention: out[b, h] = sum_t softmax_t(scale * q[b, h] . k[b, h / G, t]) v[b, h / G, t] over the lens[b] first rows (G = H / Hkv).
+// A wave takes 32 keys at a time of one (sample, KV head) with all G <= 16 query heads of the group as the columns of its MFMAs
+// (v_mfma_f32_16x16x32_bf16; K and V are de-quantised to bf16 in registers, which is exact):
+//   S^T [16 keys x heads] = K Q^T: lane (r = l & 15, g = l >> 4) holds key 4 (r & 3) + (r >> 2) and the dh / 4 dims of quarter g in one load;
+//     the lane's four results are then keys 4 i + g of head r;
+//   O^T [dh x heads] += V^T P^T: the same lane supplies the probabilities of the keys 4 i + g — where they already are, nothing is
+//     exchanged — and V is loaded in that order too: one instruction reads four whole rows, lane r its dh / 16 dims of them; the pairs
+//     of adjacent dims that the conversion yields are turned into pairs of keys by v_perm.
+// Softmax: running maximum and sum per wave in fp32; P is rounded to bf16 for the second product (its error, 2^-9 relative and
+// independent from key to key, is below that of the bf16 result).  The waves of a workgroup take alternate tiles and merge in LDS; the
+// workgroups of a split sample write (max, sum, unnormalised row) in fp32 and a second kernel joins them in order: no atomics.
+// Rows at and past lens[b] are never used: their scores are dropped and their scale bytes replaced, so they may hold anything.
+#include "mxfp4.h"
+
+namespace hvlm {
+namespace {
+
+constexpr int KV4_WAVES = 4;
+constexpr int KV4_TILE = 32;               // keys per wave and step
+
+// ---- append -----------------------------------------------------------------------------------------------------------------------
+// item = 8 elements (one dword of codes); four adjacent lanes share a block
+template <int DH>
+__global__ __launch_bounds__(256) void kv4_append_kernel(const bf16_t* __restrict__ qkv, long ld, unsigned char* __restrict__ kc,
+                                                         unsigned char* __restrict__ ks, unsigned char* __restrict__ vc,
+                                                         unsigned char* __restrict__ vs, const int32_t* __restrict__ start,
+                                                         const int32_t* __restrict__ count, int B, int S, long max_len, int H, int Hkv) {
+  constexpr int CH = DH / 8;
+  const long per_row = 2L * Hkv * CH, total = (long)B * S * per_row;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+    const long row = i / per_row;
+    const int r = (int)(i - row * per_row), hh = r / CH, c = r % CH;          // hh: 0 .. Hkv - 1 keys, Hkv .. 2 Hkv - 1 values
+    const int b = (int)(row / S), s = (int)(row - (long)b * S);
+    const long pos = (start ? start[b] : 0) + (long)s;
+    if (pos < 0 || pos >= max_len || (count && s >= count[b])) continue;       // (whole quads: a quad is one block of one row)
+    const u32x4 v = *reinterpret_cast<const u32x4*>(qkv + row * ld + (long)(H + hh) * DH + c * 8);
+    const unsigned sc = mx_scale_code<false>(mx_quad_max(mx_amax8(v)));
+    const bool is_v = hh >= Hkv;
+    const long slot = ((long)b * Hkv + (is_v ? hh - Hkv : hh)) * max_len + pos;
+    *reinterpret_cast<unsigned*>((is_v ? vc : kc) + slot * (DH / 2) + c * 4) = mx_quant8<false>(v, sc);
+    if ((c & 3) == 0) (is_v ? vs : ks)[slot * (DH / 32) + (c >> 2)] = (unsigned char)sc;
+  }
+}
+
+// ---- attention ----------------------------------------------------------------------------------------------------------------------
+struct Kv4Args {
+  const bf16_t* q;
+  const unsigned char *kc, *ks, *vc, *vs;
+  const int32_t* lens;
+  bf16_t* out;
+  float* ws;
+  long ldq, ldo, max_len;
+  int H, Hkv, G, splits;
+  float scale_log2;                       // softmax scale * log2(e)
+};
+
+__device__ __forceinline__ float quarter_max(float v) {                       // over the four lanes that share a head column
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float quarter_sum(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+template <int DH>
+__global__ __launch_bounds__(KV4_WAVES * 64, 2) void attn_decode_kv4_kernel(Kv4Args p) {
+  constexpr int KD = DH / 4;              // dims of a key per lane: KD / 2 bytes
+  constexpr int VD = DH / 16;             // dims of a value row per lane: VD / 2 bytes
+  constexpr int CB = DH / 2, SB = DH / 32;
+  extern __shared__ __attribute__((aligned(16))) float sm[];                  // [waves][G][DH] rows, then [waves][G] max, [waves][G] sum
+  const int t = threadIdx.x, w = t >> 6, l = t & 63, r16 = l & 15, g = l >> 4;
+  const int bh = blockIdx.x / p.splits, split = blockIdx.x - bh * p.splits;
+  const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  const long len = min((long)max(p.lens[b], 0), p.max_len);
+  // keys of this split: a whole number of rounds of the workgroup
+  const long round = KV4_WAVES * KV4_TILE;
+  const long per = ((len + p.splits - 1) / p.splits + round - 1) / round * round;
+  const long k0 = min(per * split, len), k1 = min(k0 + per, len);
+  const long base = (long)bh * p.max_len;
+  const unsigned char *kc = p.kc + base * CB, *ks = p.ks + base * SB, *vc = p.vc + base * CB, *vs = p.vs + base * SB;
+
+  bf16x8 qf[KD / 8];
+  {
+    const bf16_t* qp = p.q + (long)b * p.ldq + (long)(hk * p.G + min(r16, p.G - 1)) * DH + g * KD;   // (columns past G repeat the last head)
+#pragma unroll
+    for (int j = 0; j < KD / 8; ++j) qf[j] = *reinterpret_cast<const bf16x8*>(qp + j * 8);
+  }
+  f32x4 o[VD];
+#pragma unroll
+  for (int j = 0; j < VD; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float mx = -INFINITY, sum = 0.f;
+
+  const int krow = 4 * (r16 & 3) + (r16 >> 2);
+  for (long kt = k0 + w * KV4_TILE; kt < k1; kt += round) {
+    const int left = (int)min(k1 - kt, (long)KV4_TILE);                        // valid keys of this tile
+    // loads: two K tiles of 16 keys, eight V instructions of four keys (rows past the end repeat the last one)
+    unsigned kq[2][KD / 8], vq[8];
+    unsigned kb[2], vb[8];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const long key = kt + min(16 * u + krow, left - 1);
+      __builtin_memcpy(kq[u], __builtin_assume_aligned(kc + key * CB + g * (KD / 2), KD / 2), KD / 2);
+      kb[u] = ks[key * SB + g * KD / 32];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const long key = kt + min(16 * (e >> 2) + 4 * (e & 3) + g, left - 1);
+      if constexpr (VD == 8) vq[e] = *reinterpret_cast<const unsigned*>(vc + key * CB + r16 * 4);
+      else vq[e] = *reinterpret_cast<const unsigned short*>(vc + key * CB + r16 * 2);
+      vb[e] = vs[key * SB + r16 * VD / 32];
+    }
+    // scores: lane holds keys 16 u + 4 i + g of head r16
+    float s[8];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float sc = mx_scale(kb[u]);
+      f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < KD / 8; ++j) a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_bf16x8(kq[u][j], sc), qf[j], a, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[4 * u + i] = 16 * u + 4 * i + g < left ? a[i] * p.scale_log2 : -INFINITY;
+    }
+    float tm = s[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) tm = fmaxf(tm, s[e]);
+    const float nm = fmaxf(mx, quarter_max(tm));
+    const float off = nm == -INFINITY ? 0.f : nm;                              // nothing but -inf so far: every p is 0
+    const float fac = __builtin_amdgcn_exp2f(mx - off);
+    mx = nm;
+    float pr[8], ps = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { pr[e] = __builtin_amdgcn_exp2f(s[e] - off); ps += pr[e]; }
+    sum = sum * fac + ps;                                                      // (this lane's quarter of the keys; joined at the end)
+    const u32x4 pw = {pack_bf2(pr[0], pr[1]), pack_bf2(pr[2], pr[3]), pack_bf2(pr[4], pr[5]), pack_bf2(pr[6], pr[7])};
+    const bf16x8 pf = __builtin_bit_cast(bf16x8, pw);
+#pragma unroll
+    for (int j = 0; j < VD; ++j) o[j] *= fac;
+    // values: dims r16 * VD + j of the keys of quarter g; a key past the end has p = 0 and must be finite
+    unsigned vp[VD / 2][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float sc = mx_scale(16 * (e >> 2) + 4 * (e & 3) + g < left ? vb[e] : 127u);
+      vp[0][e] = mx_pair_bf16<0>(vq[e], sc);
+      vp[1][e] = mx_pair_bf16<1>(vq[e], sc);
+      if constexpr (VD == 8) { vp[2][e] = mx_pair_bf16<2>(vq[e], sc); vp[3][e] = mx_pair_bf16<3>(vq[e], sc); }
+    }
+#pragma unroll
+    for (int j = 0; j < VD; ++j) {
+      u32x4 f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        f[e] = __builtin_amdgcn_perm(vp[j >> 1][2 * e + 1], vp[j >> 1][2 * e], (j & 1) ? 0x07060302u : 0x05040100u);
+      o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, f), pf, o[j], 0, 0, 0);
+    }
+  }
+  sum = quarter_sum(sum);
+
+  // merge: lane holds dims (4 g + i) VD + j of head r16
+  float* sm_m = sm + KV4_WAVES * p.G * DH;
+  float* sm_l = sm_m + KV4_WAVES * p.G;
+  if (r16 < p.G) {
+    float* row = sm + (w * p.G + r16) * DH + 4 * g * VD;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < VD; ++j) row[i * VD + j] = o[j][i];
+    if (g == 0) { sm_m[w * p.G + r16] = mx; sm_l[w * p.G + r16] = sum; }
+  }
+  __syncthreads();
+  for (int i = t; i < p.G * DH; i += KV4_WAVES * 64) {
+    const int h = i / DH, d = i - h * DH;
+    float m = sm_m[h];
+#pragma unroll
+    for (int v = 1; v < KV4_WAVES; ++v) m = fmaxf(m, sm_m[v * p.G + h]);
+    const float off = m == -INFINITY ? 0.f : m;
+    float acc = 0.f, den = 0.f;
+#pragma unroll
+    for (int v = 0; v < KV4_WAVES; ++v) {
+      const float f = __builtin_amdgcn_exp2f(sm_m[v * p.G + h] - off);
+      acc += f * sm[(v * p.G + h) * DH + d];
+      den += f * sm_l[v * p.G + h];
+    }
+    const long head = (long)b * p.H + hk * p.G + h;
+    if (p.splits == 1) {
+      p.out[(long)b * p.ldo + (hk * p.G + h) * DH + d] = f2bf(den == 0.f ? 0.f : acc / den);
+    } else {
+      float* rec = p.ws + (head * p.splits + split) * (DH + 2);
+      rec[d] = acc;
+      if (d == 0) { rec[DH] = m; rec[DH + 1] = den; }
+    }
+  }
+}
+
+// joins the splits of one head: a workgroup of DH threads
+template <int DH>
+__global__ __launch_bounds__(DH) void kv4_combine_kernel(const float* __restrict__ ws, bf16_t* __restrict__ out, long ldo, int H, int splits) {
+  const long head = blockIdx.x;
+  const float* rec = ws + head * splits * (DH + 2);
+  const int d = threadIdx.x;
+  float m = -INFINITY;
+  for (int s = 0; s < splits; ++s) m = fmaxf(m, rec[s * (DH + 2) + DH]);
+  const float off = m == -INFINITY ? 0.f : m;
+  float acc = 0.f, den = 0.f;
+  for (int s = 0; s < splits; ++s) {
+    const float f = __builtin_amdgcn_exp2f(rec[s * (DH + 2) + DH] - off);
+    acc += f * rec[s * (DH + 2) + d];
+    den += f * rec[s * (DH + 2) + DH + 1];
+  }
+  out[(head / H) * ldo + (head % H) * DH + d] = f2bf(den == 0.f ? 0.f : acc / den);
+}
+
+// splits of the key axis: enough workgroups for four on every CU, but no split shorter than one round of a workgroup
+int kv4_splits(int B, int Hkv, long max_len) {
+  const long pairs = (long)B * Hkv, rounds = (max_len + KV4_WAVES * KV4_TILE - 1) / (KV4_WAVES * KV4_TILE);
+  long s = (1024 + pairs - 1) / pairs;
+  if (s > rounds) s = rounds;
+  return (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+}
+
+}  // namespace
+}  // namespace hvlm
+
+using namespace hvlm;
+
+static int kv4_check(const char* what, const void* kc, const void* ks, const void* vc, const void* vs, int B, long max_len, int H, int Hkv, int dh) {
+  HVLM_REQUIRE(kc && ks && vc && vs, "%s: null pointer", what);
+  HVLM_REQUIRE(B > 0 && max_len > 0 && H > 0 && Hkv > 0, "%s: B=%d, max_len=%ld, H=%d, Hkv=%d must be positive", what, B, max_len, H, Hkv);
+  HVLM_REQUIRE(dh == 64 || dh == 128, "%s: head dimension %d (64 or 128)", what, dh);
+  HVLM_REQUIRE(max_len < (1L << 31) && (long)B * Hkv < (1L << 22), "%s: cache too large", what);
+  HVLM_REQUIRE((((uintptr_t)kc | (uintptr_t)vc) & 15) == 0, "%s: codes must be 16-byte aligned", what);
+  return HVLM_OK;
+}
+
+extern "C" int hvlm_kv4_append(const void* qkv, long ld, void* k_codes, void* k_scales, void* v_codes, void* v_scales, const int32_t* start,
+                               const int32_t* count, int B, int S, long max_len, int H, int Hkv, int dh, void* stream) {
+  const int rc = kv4_check("kv4_append", k_codes, k_scales, v_codes, v_scales, B, max_len, H, Hkv, dh);
+  if (rc) return rc;
+  HVLM_REQUIRE(qkv && S > 0, "kv4_append: null rows or S=%d", S);
+  HVLM_REQUIRE(ld >= (long)(H + 2 * Hkv) * dh && ld % 8 == 0 && ((uintptr_t)qkv & 15) == 0, "kv4_append: rows must be 16-byte aligned");
+  const long total = (long)B * S * 2 * Hkv * (dh / 8), g = (total + 255) / 256;
+  const auto k = dh == 128 ? kv4_append_kernel<128> : kv4_append_kernel<64>;
+  hipLaunchKernelGGL(k, dim3((unsigned)(g < 8192 ? g : 8192)), dim3(256), 0, as_stream(stream), (const bf16_t*)qkv, ld, (unsigned char*)k_codes,
+                     (unsigned char*)k_scales, (unsigned char*)v_codes, (unsigned char*)v_scales, start, count, B, S, max_len, H, Hkv);
+  return check_launch("kv4_append");
+}
+
+extern "C" size_t hvlm_attn_decode_kv4_ws_bytes(int B, int H, int Hkv, int dh, long max_len) {
+  if (B <= 0 || H <= 0 || Hkv <= 0 || dh <= 0 || max_len <= 0) return 0;
+  const int s = kv4_splits(B, Hkv, max_len);
+  return s == 1 ? 0 : (size_t)B * H * s * (dh + 2) * 4;
+}
+
+extern "C" int hvlm_attn_decode_kv4(const void* q, long ldq, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
+                                    const int32_t* lens, void* out, long ldo, int B, long max_len, int H, int Hkv, int dh, float scale, void* ws,
+                                    void* stream) {
+  const int rc = kv4_check("attn_decode_kv4", k_codes, k_scales, v_codes, v_scales, B, max_len, H, Hkv, dh);
+  if (rc) return rc;
+  HVLM_REQUIRE(q && lens && out, "attn_decode_kv4: null pointer");
+  HVLM_REQUIRE(H % Hkv == 0 && H / Hkv <= 16, "attn_decode_kv4: H=%d must be 1 to 16 times Hkv=%d", H, Hkv);
+  HVLM_REQUIRE(ldq >= (long)H * dh && ldq % 8 == 0 && ((uintptr_t)q & 15) == 0, "attn_decode_kv4: rows of q must be 16-byte aligned");
+  HVLM_REQUIRE(ldo >= (long)H * dh, "attn_decode_kv4: leading dimension of out");
+  const int splits = kv4_splits(B, Hkv, max_len), G = H / Hkv;
+  HVLM_REQUIRE(splits == 1 || (ws && ((uintptr_t)ws & 15) == 0), "attn_decode_kv4: a 16-byte aligned workspace of hvlm_attn_decode_kv4_ws_bytes() is needed");
+  Kv4Args p{};
+  p.q = (const bf16_t*)q; p.kc = (const unsigned char*)k_codes; p.ks = (const unsigned char*)k_scales; p.vc = (const unsigned char*)v_codes;
+  p.vs = (const unsigned char*)v_scales; p.lens = lens; p.out = (bf16_t*)out; p.ws = (float*)ws; p.ldq = ldq; p.ldo = ldo; p.max_len = max_len;
+  p.H = H; p.Hkv = Hkv; p.G = G; p.splits = splits; p.scale_log2 = scale * 1.4426950408889634f;
+  const size_t lds = (size_t)KV4_WAVES * G * (dh + 2) * 4;                     // at most 33 280 bytes
+  const auto k = dh == 128 ? attn_decode_kv4_kernel<128> : attn_decode_kv4_kernel<64>;
+  hipLaunchKernelGGL(k, dim3((unsigned)(B * Hkv * splits)), dim3(KV4_WAVES * 64), lds, as_stream(stream), p);
+  const int rc2 = check_launch("attn_decode_kv4");
+  if (rc2 || splits == 1) return rc2;
+  const auto c = dh == 128 ? kv4_combine_kernel<128> : kv4_combine_kernel<64>;
+  hipLaunchKernelGGL(c, dim3((unsigned)(B * H)), dim3(dh), 0, as_stream(stream), (const float*)ws, (bf16_t*)out, ldo, H, splits);
+  return check_launch("attn_decode_kv4");
+}

@@ -40,7 +40,8 @@ extern "C" {
  * fails its version check instead of binding a different function set.
  *   1: rounds 1-3.
  *   2: round 4 (hvlm_gemm_set_sched_ws replaced by hvlm_create / hvlm_destroy, hvlm_debug_occupy left production builds,
- *      hvlm_patch_im2col_f16 and hvlm_temporal_spatial_pool_fwd_f16 added) and round 5 (library switch "attn_fwd_asm"). */
+ *      hvlm_patch_im2col_f16 and hvlm_temporal_spatial_pool_fwd_f16 added) and round 5 (library switch "attn_fwd_asm").
+ *      The MXFP4 entry points joined version 2: nothing that a host bound before changed. */
 #define HVLM_ABI_VERSION 2
 
 int hvlm_abi_version(void);
@@ -488,6 +489,48 @@ int hvlm_add_bf16(const void* a, const void* b, void* y, long n, void* stream);
 /* f32 -> bf16 and bf16 -> f32 casts (n elements). */
 int hvlm_cast_f32_to_bf16(const float* in, void* out, long n, void* stream);
 int hvlm_cast_bf16_to_f32(const void* in, float* out, long n, void* stream);
+
+/* ------------------------------------------------------------------------------------------ *
+ * Generation in 4 bits (OCP Microscaling MXFP4): 32 consecutive elements of a row share one power-of-two scale.  The reference's
+ * `--load-4bit` (handsonvlm/evaluation/evaluate.py:18-26 -> builder.py) stands for a third-party loader; there is no arithmetic of
+ * its own to match, parity = the definition below in 64 bits.
+ *   codes  : 4-bit E2M1 {0, 0.5, 1, 1.5, 2, 3, 4, 6} with a sign bit, two per byte, the even element in the low nibble: K / 2 bytes a row
+ *   scales : one E8M0 byte s per 32 elements, 2^(s - 127); 255 = the whole block is NaN: K / 32 bytes a row, at any alignment
+ *   value  : code * 2^(s - 127)
+ * Leading dimensions of codes and scales are in BYTES.  Every K is a multiple of 32.
+ * ------------------------------------------------------------------------------------------ */
+/* x [rows, K] (bf16, or IEEE half when f16 != 0; ldx elements) -> codes, scales: s - 127 = floor(log2(max |x|)) - 2 (at least -127),
+ * elements round to nearest even and saturate at 6; a block that holds an infinity or a NaN becomes NaN.  Rows of x are 16-byte,
+ * rows of codes 4-byte aligned; rows * K / 8 < 2^31. */
+int hvlm_quantize_mxfp4(const void* x, void* codes, void* scales, int rows, int K, long ldx, long ld_codes, long ld_scales, int f16,
+                        void* stream);
+/* The values back as bf16 (exact) or IEEE half (f16 != 0; rounds, overflows to infinity). */
+int hvlm_dequantize_mxfp4(const void* codes, const void* scales, void* out, int rows, int K, long ld_codes, long ld_scales, long ldo,
+                          int f16, void* stream);
+/* C[M, N] = act(A[M, K] @ B[N, K]^T + bias[N]) + residual[M, N], both operands MXFP4, fp32 accumulation on the scaled MFMA.  C is bf16, or
+ * float32 when out_f32 != 0; bias / residual are bf16 or NULL.  Any M, N; rows of codes 16-byte aligned, below 4 MiB.  residual may be C
+ * itself. */
+int hvlm_gemm_mxfp4_nt(const void* A, const void* a_scale, const void* B, const void* b_scale, void* C, int M, int N, int K, long lda,
+                       long ldas, long ldb, long ldbs, long ldc, const void* bias, const void* residual, long ldr, int act, int out_f32,
+                       void* stream);
+/* The weight-streaming form for M <= 32 (decode steps): x [M, K] in bf16 against MXFP4 weights, C in bf16.  ws: 16-byte aligned,
+ * hvlm_gemm_w4a16_ws_bytes(M, N, K) bytes, not initialised, used until the call's work on `stream` is done. */
+size_t hvlm_gemm_w4a16_ws_bytes(int M, int N, int K);
+int hvlm_gemm_w4a16_nt(const void* x, const void* W, const void* w_scale, void* C, int M, int N, int K, long ldx, long ldw, long ldws,
+                       long ldc, const void* bias, const void* residual, long ldr, int act, void* ws, void* stream);
+/* KV cache in MXFP4, per K and V: codes [B, Hkv, max_len, dh / 2], scales [B, Hkv, max_len, dh / 32], dense (one head's rows are contiguous;
+ * blocks run along the head dimension).  dh = 64 or 128; codes 16-byte aligned.
+ *   append: row (b, s) of qkv [B * S, ld] (q | k | v columns: H, Hkv and Hkv heads; k after RoPE) -> cache row start[b] + s of sample b.
+ *       start (NULL: 0) and count (NULL: S; rows s >= count[b] are skipped) are device int32 [B]; rows outside the cache are dropped.
+ *   attn_decode: out[b, h] = softmax(scale * q[b, h] . K)[t < lens[b]] V for one query row per sample; head h reads KV head
+ *       h / (H / Hkv), H / Hkv <= 16.  lens: device int32 [B], clamped to 0 .. max_len; a sample of length 0 gives zeros.  Cache rows at and
+ *       past lens[b] are never used, whatever they hold.  ws: as above, hvlm_attn_decode_kv4_ws_bytes() bytes (0: may be NULL). */
+int hvlm_kv4_append(const void* qkv, long ld, void* k_codes, void* k_scales, void* v_codes, void* v_scales, const int32_t* start,
+                    const int32_t* count, int B, int S, long max_len, int H, int Hkv, int dh, void* stream);
+size_t hvlm_attn_decode_kv4_ws_bytes(int B, int H, int Hkv, int dh, long max_len);
+int hvlm_attn_decode_kv4(const void* q, long ldq, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
+                         const int32_t* lens, void* out, long ldo, int B, long max_len, int H, int Hkv, int dh, float scale, void* ws,
+                         void* stream);
 
 #ifdef __cplusplus
 }
