@@ -356,89 +356,121 @@ def gemm_skinny_qkv(a: torch.Tensor, w_qkv, cache: torch.Tensor, lens: torch.Ten
 MX_BLOCK = 32
 
 
-def _here(name: str, *tensors):
-    """Every tensor is on the current device: its stream is the one that the launch goes to."""
-    dev = torch.cuda.current_device() if torch.cuda.is_available() else -1
+U8, F16, F32, I32 = torch.uint8, torch.float16, torch.float32, torch.int32
+
+
+def _fail(msg: str):
+    raise _lib.HvlmError(msg)
+
+
+def _launch_stream(name: str, *tensors) -> int:
+    """The current stream of the current device, on which every tensor has to be: a launch goes to that device, whatever the tensors say.
+    (The raw handle: these calls are a few microseconds long, a Stream object would be a good part of them.)"""
+    dev = -1
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device.index != dev):
-            raise _lib.HvlmError(f"{name}: expected tensors on the current device cuda:{dev}, got {t.device} (the HIP path has no CPU fallback)")
+        if t is not None:
+            d = t.get_device()
+            if dev < 0:
+                dev = d
+            if d < 0 or d != dev or d != torch._C._cuda_getDevice():
+                _fail(f"{name}: expected tensors on the current device, got {t.device} (the HIP path has no CPU fallback)")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _refuse(cond: bool, msg: str):
-    if not cond:
-        raise _lib.HvlmError(msg)
+def _ld(t: torch.Tensor) -> int:
+    """Row stride of a matrix with contiguous rows; a single row may carry any (torch leaves the stride of a dimension of 1 open)."""
+    st, shape = t.stride(), t.shape
+    if shape[1] > 1 and st[1] != 1:
+        return -1
+    return st[0] if shape[0] > 1 else shape[1]
 
 
 def _mx_pair(name: str, q):
-    """Checks an MXFP4 matrix; returns (codes, scales, rows, K)."""
+    """Checks an MXFP4 matrix; returns (codes, scales, rows, K, row stride of the codes, of the scales)."""
     codes, scales = q
-    _refuse(codes.dtype == torch.uint8 and scales.dtype == torch.uint8 and codes.dim() == 2 and scales.dim() == 2
-            and codes.shape[0] == scales.shape[0] and codes.shape[1] == scales.shape[1] * (MX_BLOCK // 2),
-            f"{name}: an MXFP4 matrix is (codes uint8 [R, K / 2], scales uint8 [R, K / 32]), got {tuple(codes.shape)} {codes.dtype}, "
-            f"{tuple(scales.shape)} {scales.dtype}")
-    _refuse((codes.shape[1] == 0 or codes.stride(1) == 1) and (scales.shape[1] <= 1 or scales.stride(1) == 1),
-            f"{name}: rows of codes and scales must be contiguous")
-    return codes, scales, codes.shape[0], codes.shape[1] * 2
-
-
-def _mx_ld(t: torch.Tensor) -> int:
-    """Row stride; a single row may carry any (torch leaves the stride of a dimension of 1 open)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    cs, ss = codes.shape, scales.shape
+    if codes.dtype != U8 or scales.dtype != U8 or len(cs) != 2 or len(ss) != 2 or cs[0] != ss[0] or cs[1] != 16 * ss[1]:
+        _fail(f"{name}: an MXFP4 matrix is (codes uint8 [R, K / 2], scales uint8 [R, K / 32]), got {codes.dtype} {tuple(cs)}, {scales.dtype} {tuple(ss)}")
+    ldc, lds = _ld(codes), _ld(scales)
+    if ldc < 0 or lds < 0:
+        _fail(f"{name}: rows of codes and scales must be contiguous")
+    return codes, scales, cs[0], 2 * cs[1], ldc, lds
 
 
 def quantize_mxfp4(x: torch.Tensor, out=None):
     """bf16 / fp16 [R, K] (row-strided, K % 32 == 0) -> (codes uint8 [R, K / 2], scales uint8 [R, K / 32]): E2M1 elements under one
     power-of-two scale per 32 (include/hvlm.h)."""
-    _refuse(x.dtype in (BF16, torch.float16) and x.dim() == 2 and x.stride(1) == 1,
-            f"quantize_mxfp4: expected a bf16 or fp16 matrix with contiguous rows, got {x.dtype} {tuple(x.shape)} {x.stride()}")
+    dt = x.dtype
+    if (dt != BF16 and dt != F16) or x.dim() != 2:
+        _fail(f"quantize_mxfp4: expected a bf16 or fp16 matrix, got {dt} {tuple(x.shape)}")
     R, K = x.shape
-    _refuse(R > 0 and K > 0 and K % MX_BLOCK == 0, f"quantize_mxfp4: R={R} must be positive, K={K} a positive multiple of {MX_BLOCK}")
+    ldx = _ld(x)
+    if ldx < 0:
+        _fail(f"quantize_mxfp4: expected contiguous rows, got strides {x.stride()}")
+    if R <= 0 or K <= 0 or K % MX_BLOCK:
+        _fail(f"quantize_mxfp4: R={R} must be positive, K={K} a positive multiple of {MX_BLOCK}")
     if out is None:
-        out = (torch.empty((R, K // 2), dtype=torch.uint8, device=x.device), torch.empty((R, K // MX_BLOCK), dtype=torch.uint8, device=x.device))
-    codes, scales, r, k = _mx_pair("quantize_mxfp4.out", out)
-    _refuse((r, k) == (R, K), f"quantize_mxfp4: out is for [{r}, {k}], x is [{R}, {K}]")
-    _here("quantize_mxfp4", x, codes, scales)
-    check(_lib.load().hvlm_quantize_mxfp4(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), R, K, _mx_ld(x), _mx_ld(codes), _mx_ld(scales),
-                                          1 if x.dtype == torch.float16 else 0, _stream()), "quantize_mxfp4")
+        dev = x.device
+        codes, scales = torch.empty((R, K // 2), dtype=U8, device=dev), torch.empty((R, K // MX_BLOCK), dtype=U8, device=dev)
+        ldc, lds = K // 2, K // MX_BLOCK
+    else:
+        codes, scales, r, k, ldc, lds = _mx_pair("quantize_mxfp4.out", out)
+        if r != R or k != K:
+            _fail(f"quantize_mxfp4: out is for [{r}, {k}], x is [{R}, {K}]")
+    stream = _launch_stream("quantize_mxfp4", x, codes, scales)
+    check(_lib.load().hvlm_quantize_mxfp4(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), R, K, ldx, ldc, lds, 1 if dt == F16 else 0, stream),
+          "quantize_mxfp4")
     return codes, scales
 
 
 def dequantize_mxfp4(q, out_dtype=BF16) -> torch.Tensor:
     """(codes, scales) -> [R, K] values in bf16 (exact) or fp16."""
-    codes, scales, R, K = _mx_pair("dequantize_mxfp4", q)
-    _refuse(out_dtype in (BF16, torch.float16), f"dequantize_mxfp4: bf16 or fp16, not {out_dtype}")
-    _here("dequantize_mxfp4", codes, scales)
+    codes, scales, R, K, ldc, lds = _mx_pair("dequantize_mxfp4", q)
+    if out_dtype != BF16 and out_dtype != F16:
+        _fail(f"dequantize_mxfp4: bf16 or fp16, not {out_dtype}")
     out = torch.empty((R, K), dtype=out_dtype, device=codes.device)
-    check(_lib.load().hvlm_dequantize_mxfp4(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), R, K, _mx_ld(codes), _mx_ld(scales), K,
-                                            1 if out_dtype == torch.float16 else 0, _stream()), "dequantize_mxfp4")
+    stream = _launch_stream("dequantize_mxfp4", codes, scales, out)
+    check(_lib.load().hvlm_dequantize_mxfp4(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), R, K, ldc, lds, K, 1 if out_dtype == F16 else 0, stream),
+          "dequantize_mxfp4")
     return out
 
 
-def _epilogue_args(name: str, M: int, N: int, dev, bias, residual, out, dtypes):
-    """Checks the optional bias / residual / output of a product; returns the residual's row stride."""
-    _refuse(bias is None or (bias.dtype == BF16 and bias.shape == (N,) and bias.is_contiguous()), f"{name}: bias must be a contiguous bf16 [{N}]")
-    _refuse(residual is None or (residual.dtype == BF16 and residual.shape == (M, N) and (N == 1 or residual.stride(1) == 1)),
-            f"{name}: residual must be bf16 [{M}, {N}] with contiguous rows")
-    _refuse(out.dtype in dtypes and out.shape == (M, N) and (N == 1 or out.stride(1) == 1), f"{name}: out must be [{M}, {N}] with contiguous rows, one of {dtypes}")
-    return 0 if residual is None else _mx_ld(residual)
+def _mx_epilogue(name: str, M: int, N: int, bias, residual):
+    """Checks the optional bias / residual of a product; returns their addresses and the residual's row stride."""
+    pb = pr = None
+    ldr = 0
+    if bias is not None:
+        if bias.dtype != BF16 or bias.shape != (N,) or not bias.is_contiguous():
+            _fail(f"{name}: bias must be a contiguous bf16 [{N}], got {bias.dtype} {tuple(bias.shape)}")
+        pb = bias.data_ptr()
+    if residual is not None:
+        if residual.dtype != BF16 or residual.shape != (M, N) or _ld(residual) < 0:
+            _fail(f"{name}: residual must be bf16 [{M}, {N}] with contiguous rows, got {residual.dtype} {tuple(residual.shape)}")
+        pr, ldr = residual.data_ptr(), _ld(residual)
+    return pb, pr, ldr
 
 
 def gemm_mxfp4_nt(a4, b4, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None, act: int = ACT_NONE,
                   out: Optional[torch.Tensor] = None, out_dtype=BF16) -> torch.Tensor:
     """out[M,N] = act(a @ b^T + bias) + residual for two MXFP4 matrices (codes, scales), [M, K] and [N, K]; bf16 or float32 out."""
-    ac, asc, M, K = _mx_pair("gemm_mxfp4.a", a4)
-    bc, bsc, N, kb = _mx_pair("gemm_mxfp4.b", b4)
-    _refuse(K == kb, f"gemm_mxfp4: a has K={K}, b has K={kb}")
+    ac, asc, M, K, lda, ldas = _mx_pair("gemm_mxfp4.a", a4)
+    bc, bsc, N, kb, ldb, ldbs = _mx_pair("gemm_mxfp4.b", b4)
+    if K != kb:
+        _fail(f"gemm_mxfp4: a has K={K}, b has K={kb}")
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=ac.device)
-    ldr = _epilogue_args("gemm_mxfp4", M, N, ac.device, bias, residual, out, (BF16, torch.float32))
-    _here("gemm_mxfp4", ac, asc, bc, bsc, bias, residual, out)
+        out, ldc = torch.empty((M, N), dtype=out_dtype, device=ac.device), N
+    else:
+        ldc = _ld(out) if out.shape == (M, N) else -1
+    dt = out.dtype
+    if ldc < 0 or (dt != BF16 and dt != F32):
+        _fail(f"gemm_mxfp4: out must be bf16 or float32 [{M}, {N}] with contiguous rows, got {dt} {tuple(out.shape)}")
+    pb, pr, ldr = _mx_epilogue("gemm_mxfp4", M, N, bias, residual)
+    stream = _launch_stream("gemm_mxfp4", ac, asc, bc, bsc, bias, residual, out)
     hook = _gemm_hook
     if hook is not None:
         hook(M, N, K, True)
-    check(_lib.load().hvlm_gemm_mxfp4_nt(ac.data_ptr(), asc.data_ptr(), bc.data_ptr(), bsc.data_ptr(), out.data_ptr(), M, N, K, _mx_ld(ac), _mx_ld(asc),
-                                         _mx_ld(bc), _mx_ld(bsc), _mx_ld(out), _p(bias), _p(residual), ldr, act,
-                                         1 if out.dtype == torch.float32 else 0, _stream()), "gemm_mxfp4_nt")
+    check(_lib.load().hvlm_gemm_mxfp4_nt(ac.data_ptr(), asc.data_ptr(), bc.data_ptr(), bsc.data_ptr(), out.data_ptr(), M, N, K, lda, ldas, ldb, ldbs, ldc,
+                                         pb, pr, ldr, act, 1 if dt == F32 else 0, stream), "gemm_mxfp4_nt")
     if hook is not None:
         hook(M, N, K, False)
     return out
@@ -448,21 +480,26 @@ def gemm_w4a16_nt(a: torch.Tensor, b4, bias: Optional[torch.Tensor] = None, resi
                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out[M,N] = act(a[M,K] @ b^T + bias) + residual for M <= 32: bf16 activations against an MXFP4 weight (codes, scales) on the
     weight-streaming kernel (decode steps)."""
-    _chk(a, BF16, "gemm_w4a16.a")
-    bc, bsc, N, K = _mx_pair("gemm_w4a16.b", b4)
-    _refuse(a.dim() == 2 and a.shape[1] == K and a.stride(1) == 1, f"gemm_w4a16: a must be [M, {K}] with contiguous rows, got {tuple(a.shape)} {a.stride()}")
+    bc, bsc, N, K, ldb, ldbs = _mx_pair("gemm_w4a16.b", b4)
+    if a.dtype != BF16 or a.dim() != 2 or a.shape[1] != K or _ld(a) < 0:
+        _fail(f"gemm_w4a16: a must be bf16 [M, {K}] with contiguous rows, got {a.dtype} {tuple(a.shape)} {a.stride()}")
     M = a.shape[0]
     if out is None:
-        out = torch.empty((M, N), dtype=BF16, device=a.device)
-    ldr = _epilogue_args("gemm_w4a16", M, N, a.device, bias, residual, out, (BF16,))
-    _here("gemm_w4a16", a, bc, bsc, bias, residual, out)
+        out, ldc = torch.empty((M, N), dtype=BF16, device=a.device), N
+    else:
+        ldc = _ld(out) if out.shape == (M, N) and out.dtype == BF16 else -1
+        if ldc < 0:
+            _fail(f"gemm_w4a16: out must be bf16 [{M}, {N}] with contiguous rows, got {out.dtype} {tuple(out.shape)}")
+    pb, pr, ldr = _mx_epilogue("gemm_w4a16", M, N, bias, residual)
+    stream = _launch_stream("gemm_w4a16", a, bc, bsc, bias, residual, out)
     lib = _lib.load()
     hook = _gemm_hook
     if hook is not None:
         hook(M, N, K, True)
-    ws = torch.empty((lib.hvlm_gemm_w4a16_ws_bytes(M, N, K),), dtype=torch.uint8, device=a.device)
-    check(lib.hvlm_gemm_w4a16_nt(a.data_ptr(), bc.data_ptr(), bsc.data_ptr(), out.data_ptr(), M, N, K, _mx_ld(a), _mx_ld(bc), _mx_ld(bsc), _mx_ld(out),
-                                 _p(bias), _p(residual), ldr, act, ws.data_ptr(), _stream()), "gemm_w4a16_nt")
+    nws = lib.hvlm_gemm_w4a16_ws_bytes(M, N, K)
+    ws = torch.empty((nws,), dtype=U8, device=a.device) if nws else None
+    check(lib.hvlm_gemm_w4a16_nt(a.data_ptr(), bc.data_ptr(), bsc.data_ptr(), out.data_ptr(), M, N, K, _ld(a), ldb, ldbs, ldc, pb, pr, ldr, act,
+                                 ws.data_ptr() if nws else None, stream), "gemm_w4a16_nt")
     if hook is not None:
         hook(M, N, K, False)
     return out
@@ -477,49 +514,61 @@ class KV4Cache(NamedTuple):
 
     @classmethod
     def empty(cls, B: int, max_len: int, kv_heads: int, dh: int, device) -> "KV4Cache":
-        mk = lambda n: torch.empty((B, kv_heads, max_len, n), dtype=torch.uint8, device=device)  # noqa: E731
+        mk = lambda n: torch.empty((B, kv_heads, max_len, n), dtype=U8, device=device)  # noqa: E731
         return cls(mk(dh // 2), mk(dh // MX_BLOCK), mk(dh // 2), mk(dh // MX_BLOCK))
 
     def checked(self, name: str):
         """(B, Hkv, max_len, dh) of a well-formed cache."""
-        _refuse(all(t.dtype == torch.uint8 and t.dim() == 4 and t.is_contiguous() for t in self), f"{name}: a cache is four dense uint8 [B, Hkv, max_len, .] tensors")
-        B, Hkv, n, half = self.k.shape
-        want = ((B, Hkv, n, half), (B, Hkv, n, half // (MX_BLOCK // 2))) * 2
-        _refuse(tuple(tuple(t.shape) for t in self) == want, f"{name}: cache shapes {[tuple(t.shape) for t in self]}")
-        return B, Hkv, n, half * 2
+        k, ks, v, vs = self
+        shape, sshape = k.shape, ks.shape
+        for t in self:
+            if t.dtype != U8 or not t.is_contiguous():
+                _fail(f"{name}: a cache is four dense uint8 [B, Hkv, max_len, .] tensors, got {t.dtype} {tuple(t.shape)} {t.stride()}")
+        if len(shape) != 4 or v.shape != shape or vs.shape != sshape or sshape[:3] != shape[:3] or len(sshape) != 4 or shape[3] != 16 * sshape[3]:
+            _fail(f"{name}: cache shapes {[tuple(t.shape) for t in self]}")
+        return shape[0], shape[1], shape[2], 2 * shape[3]
 
 
 def kv4_append(qkv: torch.Tensor, cache: KV4Cache, start: Optional[torch.Tensor], H: int, count: Optional[torch.Tensor] = None) -> None:
     """Quantises the k | v columns of qkv [B * S, (H + 2 Hkv) dh] (fused q|k|v rows after RoPE) into rows start[b] .. start[b] + S - 1 of
     every sample of the cache (start None: 0).  count int32 [B]: only the first count[b] rows of a sample.  Rows outside the cache are
     dropped.  start / count are read on the device."""
-    _chk(qkv, BF16, "kv4_append.qkv")
     B, Hkv, n, dh = cache.checked("kv4_append")
-    _refuse(qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[1] == (H + 2 * Hkv) * dh and qkv.shape[0] % B == 0,
-            f"kv4_append: qkv {tuple(qkv.shape)} for B={B}, H={H}, Hkv={Hkv}, dh={dh}")
+    M, ld = qkv.shape[0], _ld(qkv) if qkv.dim() == 2 else -1
+    if qkv.dtype != BF16 or ld < 0 or qkv.shape[1] != (H + 2 * Hkv) * dh or M % B:
+        _fail(f"kv4_append: qkv must be bf16 rows, got {qkv.dtype} {tuple(qkv.shape)} for B={B}, H={H}, Hkv={Hkv}, dh={dh}")
     for t in (start, count):
-        _refuse(t is None or (t.dtype == torch.int32 and t.shape == (B,) and t.is_contiguous()), f"kv4_append: start / count must be int32 [{B}]")
-    _here("kv4_append", qkv, *cache, start, count)
-    check(_lib.load().hvlm_kv4_append(qkv.data_ptr(), _mx_ld(qkv), cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(),
-                                      cache.v_scale.data_ptr(), _p(start), _p(count), B, qkv.shape[0] // B, n, H, Hkv, dh, _stream()), "kv4_append")
+        if t is not None and (t.dtype != I32 or t.shape != (B,) or not t.is_contiguous()):
+            _fail(f"kv4_append: start / count must be int32 [{B}], got {t.dtype} {tuple(t.shape)}")
+    k, ks, v, vs = cache
+    stream = _launch_stream("kv4_append", qkv, k, ks, v, vs, start, count)
+    check(_lib.load().hvlm_kv4_append(qkv.data_ptr(), ld, k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(),
+                                      None if start is None else start.data_ptr(), None if count is None else count.data_ptr(), B, M // B, n, H, Hkv, dh,
+                                      stream), "kv4_append")
 
 
 def attn_decode_kv4(q: torch.Tensor, cache: KV4Cache, lens: torch.Tensor, H: int, scale: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Single-token attention over the 4-bit cache: q [B, >= H dh] (row b = the new token of sample b after RoPE; may be the fused qkv rows),
     lens int32 [B] on the device (keys 0 .. lens[b] - 1; 0 gives zeros) -> [B, H dh].  Head h reads KV head h // (H // Hkv)."""
-    _chk(q, BF16, "attn_decode_kv4.q")
     B, Hkv, n, dh = cache.checked("attn_decode_kv4")
-    _refuse(q.dim() == 2 and q.shape[0] == B and q.shape[1] >= H * dh and q.stride(1) == 1, f"attn_decode_kv4: q {tuple(q.shape)} for B={B}, H={H}, dh={dh}")
-    _refuse(lens.dtype == torch.int32 and lens.shape == (B,) and lens.is_contiguous(), f"attn_decode_kv4: lens must be int32 [{B}]")
+    ldq = _ld(q) if q.dim() == 2 else -1
+    if q.dtype != BF16 or ldq < 0 or q.shape[0] != B or q.shape[1] < H * dh:
+        _fail(f"attn_decode_kv4: q must be bf16 rows, got {q.dtype} {tuple(q.shape)} for B={B}, H={H}, dh={dh}")
+    if lens.dtype != I32 or lens.shape != (B,) or not lens.is_contiguous():
+        _fail(f"attn_decode_kv4: lens must be int32 [{B}], got {lens.dtype} {tuple(lens.shape)}")
     if out is None:
-        out = torch.empty((B, H * dh), dtype=BF16, device=q.device)
-    _refuse(out.dtype == BF16 and out.shape == (B, H * dh) and out.stride(1) == 1, f"attn_decode_kv4: out must be bf16 [{B}, {H * dh}]")
-    _here("attn_decode_kv4", q, *cache, lens, out)
+        out, ldo = torch.empty((B, H * dh), dtype=BF16, device=q.device), H * dh
+    else:
+        ldo = _ld(out) if out.shape == (B, H * dh) and out.dtype == BF16 else -1
+        if ldo < 0:
+            _fail(f"attn_decode_kv4: out must be bf16 [{B}, {H * dh}] with contiguous rows, got {out.dtype} {tuple(out.shape)}")
+    k, ks, v, vs = cache
+    stream = _launch_stream("attn_decode_kv4", q, k, ks, v, vs, lens, out)
     lib = _lib.load()
     nws = lib.hvlm_attn_decode_kv4_ws_bytes(B, H, Hkv, dh, n)
-    ws = torch.empty((nws,), dtype=torch.uint8, device=q.device) if nws else None
-    check(lib.hvlm_attn_decode_kv4(q.data_ptr(), _mx_ld(q), cache.k.data_ptr(), cache.k_scale.data_ptr(), cache.v.data_ptr(), cache.v_scale.data_ptr(),
-                                   lens.data_ptr(), out.data_ptr(), _mx_ld(out), B, n, H, Hkv, dh, float(scale), _p(ws), _stream()), "attn_decode_kv4")
+    ws = torch.empty((nws,), dtype=U8, device=q.device) if nws else None
+    check(lib.hvlm_attn_decode_kv4(q.data_ptr(), ldq, k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), lens.data_ptr(), out.data_ptr(), ldo, B, n,
+                                   H, Hkv, dh, scale, ws.data_ptr() if nws else None, stream), "attn_decode_kv4")
     return out
 
 

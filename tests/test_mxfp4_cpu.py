@@ -69,7 +69,7 @@ def test_wrapper_refusals(ops):
     refused(lambda: ops.gemm_mxfp4_nt(pair(4, 64), pair(5, 64), out=torch.zeros(4, 5, dtype=torch.float16)), "out must be")
     refused(lambda: ops.gemm_mxfp4_nt(pair(4, 64), pair(5, 64)), "current device")
     refused(lambda: ops.gemm_w4a16_nt(x.float(), pair(5, 64)), "a")
-    refused(lambda: ops.gemm_w4a16_nt(x, pair(5, 64)), "expected a GPU tensor")
+    refused(lambda: ops.gemm_w4a16_nt(x, pair(5, 64)), "current device")
 
 
 def test_cache_refusals(ops):
@@ -78,8 +78,8 @@ def test_cache_refusals(ops):
     refused(lambda: c._replace(v=c.v[:, :, :4]).checked("t"), "dense")
     refused(lambda: c._replace(v=c.v[:, :, :4].contiguous()).checked("t"), "shapes")
     refused(lambda: c._replace(k_scale=c.k_scale.float()).checked("t"), "uint8")
-    refused(lambda: ops.kv4_append(torch.zeros(2, 6 * 64, dtype=BF16), c, None, 2), "expected a GPU tensor")
-    refused(lambda: ops.attn_decode_kv4(torch.zeros(2, 128, dtype=BF16), c, torch.zeros(2, dtype=torch.int32), 2, 0.1), "expected a GPU tensor")
+    refused(lambda: ops.kv4_append(torch.zeros(2, 6 * 64, dtype=BF16), c, None, 2), "current device")
+    refused(lambda: ops.attn_decode_kv4(torch.zeros(2, 128, dtype=BF16), c, torch.zeros(2, dtype=torch.int32), 2, 0.1), "current device")
 
 
 def test_c_refusals(ops):
