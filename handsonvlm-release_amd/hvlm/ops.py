@@ -469,8 +469,11 @@ def gemm_mxfp4_nt(a4, b4, bias: Optional[torch.Tensor] = None, residual: Optiona
     hook = _gemm_hook
     if hook is not None:
         hook(M, N, K, True)
-    check(_lib.load().hvlm_gemm_mxfp4_nt(ac.data_ptr(), asc.data_ptr(), bc.data_ptr(), bsc.data_ptr(), out.data_ptr(), M, N, K, lda, ldas, ldb, ldbs, ldc,
-                                         pb, pr, ldr, act, 1 if dt == F32 else 0, stream), "gemm_mxfp4_nt")
+    lib = _lib.load()
+    nws = lib.hvlm_gemm_mxfp4_ws_bytes(M, N, K)
+    ws = torch.empty((nws,), dtype=U8, device=out.device) if nws else None
+    check(lib.hvlm_gemm_mxfp4_nt(ac.data_ptr(), asc.data_ptr(), bc.data_ptr(), bsc.data_ptr(), out.data_ptr(), M, N, K, lda, ldas, ldb, ldbs, ldc,
+                                 pb, pr, ldr, act, 1 if dt == F32 else 0, ws.data_ptr() if nws else None, stream), "gemm_mxfp4_nt")
     if hook is not None:
         hook(M, N, K, False)
     return out

@@ -509,10 +509,11 @@ int hvlm_dequantize_mxfp4(const void* codes, const void* scales, void* out, int 
                           int f16, void* stream);
 /* C[M, N] = act(A[M, K] @ B[N, K]^T + bias[N]) + residual[M, N], both operands MXFP4, fp32 accumulation on the scaled MFMA.  C is bf16, or
  * float32 when out_f32 != 0; bias / residual are bf16 or NULL.  Any M, N; rows of codes 16-byte aligned, below 4 MiB.  residual may be C
- * itself. */
+ * itself.  ws: 16-byte aligned, hvlm_gemm_mxfp4_ws_bytes(M, N, K) bytes, not initialised, used until the call's work on `stream` is done. */
+size_t hvlm_gemm_mxfp4_ws_bytes(int M, int N, int K);
 int hvlm_gemm_mxfp4_nt(const void* A, const void* a_scale, const void* B, const void* b_scale, void* C, int M, int N, int K, long lda,
                        long ldas, long ldb, long ldbs, long ldc, const void* bias, const void* residual, long ldr, int act, int out_f32,
-                       void* stream);
+                       void* ws, void* stream);
 /* The weight-streaming form for M <= 32 (decode steps): x [M, K] in bf16 against MXFP4 weights, C in bf16.  ws: 16-byte aligned,
  * hvlm_gemm_w4a16_ws_bytes(M, N, K) bytes, not initialised, used until the call's work on `stream` is done. */
 size_t hvlm_gemm_w4a16_ws_bytes(int M, int N, int K);

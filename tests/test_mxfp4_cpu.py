@@ -101,8 +101,8 @@ def test_c_refusals(ops):
     bad(lib.hvlm_quantize_mxfp4(p, p, p, 1 << 30, 32, 32, 16, 1, 0, N), "too many")
     bad(lib.hvlm_quantize_mxfp4(p, p, p, 1, 32, 32, 16, 1, 2, N), "f16")
     bad(lib.hvlm_dequantize_mxfp4(p, p, p, 1, 32, 8, 1, 32, 0, N), "codes")
-    gm = lambda A=p, M=1, N_=1, K=32, lda=16, ldas=1, ldc=1, res=N, ldr=0, act=0, C=p: lib.hvlm_gemm_mxfp4_nt(  # noqa: E731
-        A, p, p, p, C, M, N_, K, lda, ldas, 16 * (K // 32), K // 32, ldc, N, res, ldr, act, 0, N)
+    gm = lambda A=p, M=1, N_=1, K=32, lda=16, ldas=1, ldc=1, res=N, ldr=0, act=0, C=p, ws=p: lib.hvlm_gemm_mxfp4_nt(  # noqa: E731
+        A, p, p, p, C, M, N_, K, lda, ldas, 16 * (K // 32), K // 32, ldc, N, res, ldr, act, 0, ws, N)
     bad(gm(A=N), "null")
     bad(gm(M=0), "positive")
     bad(gm(K=16), "multiple of 32")
@@ -113,6 +113,9 @@ def test_c_refusals(ops):
     bad(gm(N_=3), "leading dimensions of C")
     bad(gm(res=p), "leading dimensions of C")
     bad(gm(act=7), "act")
+    bad(gm(ws=N), "null")
+    bad(gm(ws=odd), "workspace")
+    assert lib.hvlm_gemm_mxfp4_ws_bytes(0, 4, 32) == 0 and lib.hvlm_gemm_mxfp4_ws_bytes(867, 4096, 4096) == (7 + 32) * 2 * 32 * 256
     sk = lambda M=1, K=32, ldx=32, ws=p, x=p: lib.hvlm_gemm_w4a16_nt(x, p, p, p, M, 4, K, ldx, 16 * (K // 32), K // 32, 4, N, N, 0, 0, ws, N)  # noqa: E731
     bad(sk(ws=N), "null")
     bad(sk(M=33), "1 .. 32")
