@@ -3,14 +3,21 @@
 //   C[m, n] = sum over blocks g of 2^(sa[m, g] + sb[n, g] - 254) * sum_{k in g} a[m, k] b[n, k]
 //
 // is what v_mfma_scale_f32_16x16x128_f8f6f4 computes on fp4 operands: lane (r = l & 15, q = l >> 4) holds block q (32 codes, 16 bytes) of
-// row r and that block's E8M0 byte, so a K-step of 128 takes one 16-byte LDS read and one byte of scale per fragment.  The weights are the
-// first MFMA operand: a lane's four results are four consecutive columns of one output row.
+// row r and that block's E8M0 byte, so 128 k of a fragment are one 16-byte LDS read and one byte of scale (a byte of a register that four
+// fragments share).  The weights are the first MFMA operand: a lane's four results are four consecutive columns of one output row.
 //
-// A workgroup of four waves computes a BM x BN tile, each wave a quarter.  Operand codes go from global memory to LDS without passing
-// registers (16 rows x 64 B per wave instruction, 16-byte chunks permuted by c ^ ((row >> 1) & 3) so that eight adjacent rows of a
-// fragment read fall into eight bank groups), two stages of 128 k ahead of their use; the scale bytes (4 per row and stage)
-// take the way through a register, because their rows may start at any byte.  Rows past M / N and blocks
-// past K read as zero codes.
+// Bound: the instruction issue of the four waves, one per SIMD.  A product lasts 16 cycles and the matrix pipe queues nothing behind it, so a
+// wave that issues anything longer than that between two products idles the pipe.  What follows from it:
+//   * a wave owns a quarter of the tile (128 x 128 of 256 x 256: all 256 accumulation registers) and keeps the fragments of two steps, so a
+//     step is 64 products without a wait, with the next step's 17 LDS reads and 8 LDS-DMA pieces strewn between them one at a time;
+//   * codes go from global memory to LDS by DMA in rows of 128 bytes (rows of 64 halve the L2's rate: 16.7 instead of 32 TB/s), addressed by a
+//     register that runs along, with 16-byte chunks permuted by c ^ (row & 7): eight rows of a fragment read fall into eight bank groups;
+//   * scales are tiled once per call by a kernel of their own (3 us at 22 016 rows of 4096) so that a step's fit one dword per four fragments:
+//     gathered row by row inside the K loop they cost a quarter of it (0.15 of 0.78 us a step);
+//   * workgroups are persistent and the ring runs on into the next tile, whose first 512 k land during the last of this one.
+// 13872 x 22016 x 4096: 610 us = 4.1 PFLOP/s (two groups of four waves one barrier apart, the shape of gemm_pp.hip: 723 us).  Without DMA and
+// scales a step would take 0.46 us instead of 0.62, the products alone 0.43; the rest is the tiles' ends (vision shapes with K = 1024 are
+// mostly that: 90 us where the result's bytes need 44).
 #include "mxfp4.h"
 #include <algorithm>
 #include <type_traits>
@@ -78,12 +85,19 @@ __device__ __forceinline__ void mx_epilogue(const Mx4Args& p, const f32x4 (&acc)
   constexpr bool WIDE = RES || F32;
   constexpr int TP = WIDE ? 4 : TN;                                              // fragments of a pass
   constexpr int LPR = WIDE ? 8 : 2 * TP;                                         // lanes that share a row, eight columns each
-  constexpr int RPI = 64 / LPR;                                                  // rows of one instruction
+  constexpr int RPI = 64 / LPR, NI = 16 / RPI;                                   // rows of one instruction, instructions of sixteen rows
+  constexpr int RB = WIDE ? 256 : 32 * TP, CH = RB / 16 - 1, ES = F32 ? 4 : 2;   // bytes of a row in LDS, its chunks - 1, bytes of a result
   const int l = mx_lane(), r16 = l & 15, q = l >> 4;
   const int cl = l & (LPR - 1), rl = l / LPR;                                    // this lane's columns / row behind the exchange
+  // where fragment j is written: ^ 64 j (a chunk a quarter) or ^ 32 j (half a chunk)
+  const unsigned at = r16 * RB + (WIDE ? (q ^ (r16 & CH)) * 16 : ((q >> 1) ^ (r16 & CH)) * 16 + (q & 1) * 8);
+  // where row rl + RPI k of the sixteen is read: the row's permutation differs from k to k in bits that RPI k does not share with rl
+  auto from = [&](int k, int c) { return (unsigned)((rl + RPI * k) * RB + (c ^ ((rl + RPI * k) & CH)) * 16); };
+  const int rows = p.M - m;                                                      // rows of this wave inside C
 #pragma unroll
   for (int h = 0; h < TN / TP; ++h) {
-    const int col = n + 16 * TP * h;
+    const int col = n + 16 * TP * h, cols = p.N - col;
+    const int mine = 8 * cl + 8 <= cols ? rows : 0;                              // rows whose eight columns of this lane are all inside C
     float b[TP][4];
     if constexpr (PRE > 0) {
 #pragma unroll
@@ -91,34 +105,21 @@ __device__ __forceinline__ void mx_epilogue(const Mx4Args& p, const f32x4 (&acc)
 #pragma unroll
         for (int e = 0; e < 4; ++e) b[j][e] = p.bias ? bf2f(p.bias[min(col + 16 * j + 4 * q + e, p.N - 1)]) : 0.f;
     }
-    const int c8 = col + 8 * cl;
-    const bool whole = c8 + 8 <= p.N;
-    auto residual = [&](int row) {
+    const char* const rbase = reinterpret_cast<const char*>(p.res) + ((long)m * p.ldr + col) * 2;
+    char* const cbase = reinterpret_cast<char*>(p.C) + ((long)m * p.ldc + col) * ES;
+    const unsigned rv = (unsigned)rl * (unsigned)p.ldr * 2u + cl * 16u, cv = (unsigned)rl * (unsigned)p.ldc * ES + cl * 8u * ES;
+    auto residual = [&](int i, int k) {
       u32x4 x = {0u, 0u, 0u, 0u};
-      if (row < p.M) {
-        const bf16_t* s = p.res + (long)row * p.ldr + c8;
-        if (whole) x = *reinterpret_cast<const u32x4_u*>(s);
-        else
-#pragma unroll
-          for (int e = 0; e < 8; ++e) if (c8 + e < p.N) x[e >> 1] |= (unsigned)s[e] << (16 * (e & 1));
-      }
+      if (16 * i + RPI * k + rl < mine) x = *reinterpret_cast<const u32x4_u*>(rbase + (long)(16 * i + RPI * k) * p.ldr * 2 + rv);
       return x;
     };
-    u32x4 rn[16 / RPI];                                                          // (a row's residual is read before its results are stored: C may be the residual)
+    u32x4 rn[NI];                                                                // (a row's residual is read before its results are stored: C may be the residual)
     if constexpr (RES) {
 #pragma unroll
-      for (int k = 0; k < 16 / RPI; ++k) rn[k] = residual(m + RPI * k + rl);
+      for (int k = 0; k < NI; ++k) rn[k] = residual(0, k);
     }
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-      u32x4 rc[16 / RPI];
-      if constexpr (RES) {
-#pragma unroll
-        for (int k = 0; k < 16 / RPI; ++k) {
-          rc[k] = rn[k];
-          if (i + 1 < TM) rn[k] = residual(m + 16 * (i + 1) + RPI * k + rl);
-        }
-      }
 #pragma unroll
       for (int j = 0; j < TP; ++j) {
         f32x4 v = mx_take(acc[i][TP * h + j]);
@@ -129,46 +130,53 @@ __device__ __forceinline__ void mx_epilogue(const Mx4Args& p, const f32x4 (&acc)
             if constexpr (PRE == 2) v[e] *= __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.702f * 1.4426950408889634f * v[e]));
           }
         }
-        if constexpr (WIDE) {
-          *reinterpret_cast<f32x4*>(buf + r16 * 256 + ((4 * j + q) ^ r16) * 16) = v;
-        } else {
-          constexpr int CH = 2 * TP - 1;                                         // chunks of a row - 1
-          *reinterpret_cast<u32x2*>(buf + r16 * 32 * TP + ((2 * j + (q >> 1)) ^ (r16 & CH)) * 16 + (q & 1) * 8) = u32x2{pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])};
+        if constexpr (WIDE) *reinterpret_cast<f32x4*>(buf + (at ^ (64u * j))) = v;
+        else *reinterpret_cast<u32x2*>(buf + (at ^ (32u * j))) = u32x2{pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])};
+      }
+      u32x4 rc[NI];
+      if constexpr (RES) {
+#pragma unroll
+        for (int k = 0; k < NI; ++k) {
+          rc[k] = rn[k];
+          if (i + 1 < TM) rn[k] = residual(i + 1, k);
         }
       }
 #pragma unroll
-      for (int k = 0; k < 16 / RPI; ++k) {
-        const int r = RPI * k + rl, row = m + 16 * i + r;
+      for (int k = 0; k < NI; ++k) {
+        char* const o = cbase + (long)(16 * i + RPI * k) * p.ldc * ES;
+        const bool in = 16 * i + RPI * k + rl < mine;
         if constexpr (!WIDE) {
-          constexpr int CH = 2 * TP - 1;
-          const u32x4 d = *reinterpret_cast<const u32x4*>(buf + r * 32 * TP + (cl ^ (r & CH)) * 16);
-          if (row < p.M) {
-            bf16_t* o = reinterpret_cast<bf16_t*>(p.C) + (long)row * p.ldc + c8;
-            if (whole) *reinterpret_cast<u32x4_u*>(o) = d;
-            else
-#pragma unroll
-              for (int e = 0; e < 8; ++e) if (c8 + e < p.N) o[e] = (bf16_t)(d[e >> 1] >> (16 * (e & 1)));
-          }
+          const u32x4 d = *reinterpret_cast<const u32x4*>(buf + from(k, cl));
+          if (in) *reinterpret_cast<u32x4_u*>(o + cv) = d;
         } else {
-          f32x4 x = *reinterpret_cast<const f32x4*>(buf + r * 256 + ((2 * cl) ^ r) * 16), y = *reinterpret_cast<const f32x4*>(buf + r * 256 + ((2 * cl + 1) ^ r) * 16);
+          f32x4 x = *reinterpret_cast<const f32x4*>(buf + from(k, 2 * cl)), y = *reinterpret_cast<const f32x4*>(buf + from(k, 2 * cl + 1));
           if constexpr (RES) {
             x += f32x4{bf_lo(rc[k][0]), bf_hi(rc[k][0]), bf_lo(rc[k][1]), bf_hi(rc[k][1])};
             y += f32x4{bf_lo(rc[k][2]), bf_hi(rc[k][2]), bf_lo(rc[k][3]), bf_hi(rc[k][3])};
           }
-          if (row < p.M) {
+          if (in) {
             if constexpr (F32) {
-              float* o = reinterpret_cast<float*>(p.C) + (long)row * p.ldc + c8;
-              if (whole) { *reinterpret_cast<f32x4_u*>(o) = x; *reinterpret_cast<f32x4_u*>(o + 4) = y; }
-              else
-#pragma unroll
-                for (int e = 0; e < 8; ++e) if (c8 + e < p.N) o[e] = e < 4 ? x[e & 3] : y[e & 3];
+              *reinterpret_cast<f32x4_u*>(o + cv) = x;
+              *reinterpret_cast<f32x4_u*>(o + cv + 16) = y;
             } else {
-              const u32x4 d = {pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]), pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3])};
-              bf16_t* o = reinterpret_cast<bf16_t*>(p.C) + (long)row * p.ldc + c8;
-              if (whole) *reinterpret_cast<u32x4_u*>(o) = d;
-              else
-#pragma unroll
-                for (int e = 0; e < 8; ++e) if (c8 + e < p.N) o[e] = (bf16_t)(d[e >> 1] >> (16 * (e & 1)));
+              *reinterpret_cast<u32x4_u*>(o + cv) = u32x4{pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]), pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3])};
+            }
+          }
+        }
+      }
+      if (cols > 0 && cols < 16 * TP && (cols & 7)) {                            // the last, partial eight columns of C: an element a lane
+#pragma unroll 1
+        for (int e = l; e < 128; e += 64) {
+          const int r = e >> 3, c = (cols & ~7) + (e & 7);
+          if (16 * i + r < rows && c < cols) {
+            const long row = m + 16 * i + r;
+            if constexpr (!WIDE) {
+              reinterpret_cast<bf16_t*>(p.C)[row * p.ldc + col + c] = *reinterpret_cast<const bf16_t*>(buf + r * RB + ((c >> 3) ^ (r & CH)) * 16 + (c & 7) * 2);
+            } else {
+              float x = *reinterpret_cast<const float*>(buf + r * RB + ((c >> 2) ^ (r & CH)) * 16 + (c & 3) * 4);
+              if constexpr (RES) x += bf2f(p.res[row * p.ldr + col + c]);
+              if constexpr (F32) reinterpret_cast<float*>(p.C)[row * p.ldc + col + c] = x;
+              else reinterpret_cast<bf16_t*>(p.C)[row * p.ldc + col + c] = f2bf(x);
             }
           }
         }
@@ -459,14 +467,19 @@ __global__ __launch_bounds__(256) void mx4_tile_scales_kernel(const unsigned cha
 __global__ __launch_bounds__(256, 1) void gemm_mxfp4_256_kernel(Mx4Args p) { gemm_mxfp4_body<256, 256, 1>(p); }
 __global__ __launch_bounds__(256, 1) void gemm_mxfp4_128_kernel(Mx4Args p) { gemm_mxfp4_body<128, 128, 2>(p); }
 
-// Two shapes of tile, see the table above hvlm_gemm_mxfp4_nt
+// Two shapes of tile.  A workgroup takes about 0.62 us per 128 k of a 256 x 256 tile and 3 us to write it, 0.6 us per 256 k of a 128 x 128 tile
+// and 1 us to write that; filling and draining cost 7 and 5 us once.  Rounds of 256 workgroups decide (256 / 128, microseconds measured):
+// 867 x 12288 x 4096 35.4 / 36.1, 867 x 22016 x 4096 60 / 56, 867 x 4096 x 11008 65 / 33, 2000 x 2000 x 2048 22.7 / 13.4,
+// 25700 x 4096 x 1024 92 / 109, 13872 x 22016 x 4096 610 / 760.
 struct Mx4Plan {
   int tile, qa, qb, steps;                 // quads of row tiles of A and B, 128-k steps of a row (whole groups)
   size_t ws;
 };
 Mx4Plan mx4_plan(int M, int N, int K) {
   Mx4Plan r;
-  r.tile = (long)cdiv(M, 256) * cdiv(N, 256) >= 128 ? 256 : 128;
+  const long r256 = cdiv((long)cdiv(M, 256) * cdiv(N, 256), MX_CUS), r128 = cdiv((long)cdiv(M, 128) * cdiv(N, 128), MX_CUS);
+  const long t256 = 700 + r256 * (62L * cdiv(K, 128) + 300), t128 = 500 + r128 * (60L * cdiv(K, 256) + 100);
+  r.tile = t256 < t128 ? 256 : 128;
   const int ks = r.tile == 256 ? 1 : 2;
   r.qa = cdiv(M, r.tile) * (r.tile / 64);
   r.qb = cdiv(N, r.tile) * (r.tile / 64);
@@ -503,7 +516,7 @@ extern "C" int hvlm_gemm_mxfp4_nt(const void* A, const void* a_scale, const void
                "gemm_mxfp4_nt: rows of codes must be 16-byte aligned");
   HVLM_REQUIRE(lda < (1L << 22) && ldb < (1L << 22), "gemm_mxfp4_nt: leading dimensions of the codes must be below 4 MiB");
   HVLM_REQUIRE(ldas >= K / MX_BLOCK && ldbs >= K / MX_BLOCK, "gemm_mxfp4_nt: leading dimensions of the scales");
-  HVLM_REQUIRE(ldc >= N && (!residual || ldr >= N), "gemm_mxfp4_nt: leading dimensions of C / residual");
+  HVLM_REQUIRE(ldc >= N && ldc < (1L << 26) && (!residual || (ldr >= N && ldr < (1L << 26))), "gemm_mxfp4_nt: leading dimensions of C / residual");
   HVLM_REQUIRE(act == HVLM_ACT_NONE || act == HVLM_ACT_QUICK_GELU, "gemm_mxfp4_nt: unknown act %d", act);
   HVLM_REQUIRE((long)cdiv(M, 128) * cdiv(N, 128) < (1L << 30), "gemm_mxfp4_nt: too many tiles");
   HVLM_REQUIRE(((uintptr_t)ws & 15) == 0, "gemm_mxfp4_nt: the workspace must be 16-byte aligned");
