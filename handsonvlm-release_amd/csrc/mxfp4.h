@@ -11,11 +11,8 @@ namespace hvlm {
 
 constexpr int MX_BLOCK = 32;
 
-// E8M0 byte -> the fp32 scale operand of v_cvt_scalef32_*: its exponent field, except that 2^-127 is a subnormal and 255 a NaN
-__device__ __forceinline__ float mx_scale(unsigned s) {
-  const unsigned bits = s == 0u ? 0x00400000u : s == 255u ? 0x7fc00000u : s << 23;
-  return __uint_as_float(bits);
-}
+// E8M0 byte -> the fp32 scale operand of v_cvt_scalef32_*: it reads the exponent field alone, 0 as 2^-127 and 255 as NaN
+__device__ __forceinline__ float mx_scale(unsigned s) { return __uint_as_float(s << 23); }
 
 // largest magnitude bits of a block (sign cleared: ordered like the magnitudes, infinities and NaNs on top) -> its E8M0 byte
 template <bool F16>
