@@ -26,10 +26,11 @@ def inference(model, sample: Dict, temperature=0.5, top_p=0.9, max_new_tokens=10
 
 @torch.no_grad()
 def inference_batch(model, batch, temperature=0.5, top_p=0.9, max_new_tokens=100, do_sample=True, fp8=False, pad_token_id=0,
-                    fp8_decode=False, fp8_clip=False):
+                    fp8_decode=False, fp8_clip=False, mxfp4=False, mxfp4_decode=False, kv4=False):
     """A list of samples -> list of pred_hands ([1,2,n,2] or None), generated in lock step (model.generate_batch): prompts
     are right-padded to the longest one, exactly like the reference's collator would.  fp8 / fp8_decode / fp8_clip: e4m3 prefill
-    GEMMs / e4m3-weight decode steps / e4m3 CLIP tower (all off = the reference's bf16 + fp16-tower numerics)."""
+    GEMMs / e4m3-weight decode steps / e4m3 CLIP tower (all off = the reference's bf16 + fp16-tower numerics).  mxfp4 / mxfp4_decode /
+    kv4: MXFP4 prefill GEMMs / MXFP4-weight decode steps / keys and values kept in MXFP4."""
     T = max(s["input_ids"].shape[1] for s in batch)
     ids = torch.full((len(batch), T), pad_token_id, dtype=torch.long)
     mask = torch.zeros((len(batch), T), dtype=torch.bool)
@@ -39,7 +40,8 @@ def inference_batch(model, batch, temperature=0.5, top_p=0.9, max_new_tokens=100
         mask[b, :n] = True
     image = torch.cat([s["image"] for s in batch], 0)
     out = model.generate_batch(ids, image=image, attention_mask=mask, do_sample=do_sample, temperature=temperature, top_p=top_p,
-                               max_new_tokens=max_new_tokens, fp8=fp8, fp8_decode=fp8_decode, fp8_clip=fp8_clip)
+                               max_new_tokens=max_new_tokens, fp8=fp8, fp8_decode=fp8_decode, fp8_clip=fp8_clip, mxfp4=mxfp4, mxfp4_decode=mxfp4_decode,
+                               kv4=kv4)
     return [out.pred_hands[b:b + 1, :, : out.num_hands[b]] if out.num_hands[b] > 0 else None for b in range(len(batch))]
 
 
@@ -115,6 +117,8 @@ def main(argv=None, samples=None):
     ap.add_argument("--top-p", type=float, default=0.9)
     ap.add_argument("--max-new-tokens", type=int, default=100)
     ap.add_argument("--fp8", action="store_true", help="e4m3 prefill + decode + CLIP GEMMs (BASELINE config 5; needs --batch-size > 1)")
+    ap.add_argument("--mxfp4", action="store_true", help="MXFP4 (4-bit) decoder GEMMs in prefill and decode (needs --batch-size > 1)")
+    ap.add_argument("--kv4", action="store_true", help="keys and values kept in MXFP4 while generating (needs --batch-size > 1)")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--device", default="cuda")
     a = ap.parse_args(argv)
@@ -140,6 +144,12 @@ def main(argv=None, samples=None):
         assert a.batch_size > 1, "--fp8 runs through the batched generation path"
         v = model.config.vision                      # (the e4m3 GEMM needs K % 128 == 0: every tower GEMM of ViT-L/14 qualifies)
         kw.update(fp8=True, fp8_decode=True, fp8_clip=(v.hidden_size % 128 == 0 and v.intermediate_size % 128 == 0))
+    assert not (a.fp8 and a.mxfp4), "--fp8 and --mxfp4 name two formats for the same weights"
+    if a.mxfp4:
+        kw.update(mxfp4=True, mxfp4_decode=True)
+    if a.kv4:
+        kw.update(kv4=True)
+    assert a.batch_size > 1 or not (a.mxfp4 or a.kv4), "--mxfp4 / --kv4 run through the batched generation path"
     # under torchrun every rank scores samples[rank::world] (evaluate_traj) and the predictions are all-gathered for the metric:
     # N ranks = 1/N of the work each, one metric (handsonvlm_trainer.py:241-251)
     res = evaluate_traj(model, samples, batch_size=a.batch_size, **kw)

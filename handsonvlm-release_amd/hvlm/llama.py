@@ -72,10 +72,10 @@ class LayerParams:
 
 class SeqInfo:
     """Row layout of one batch: padded (cu is None: sample b = rows [b*S, (b+1)*S)) or packed (cu int32 [B+1])."""
-    __slots__ = ("B", "S", "M", "cu", "pos", "fp8")
+    __slots__ = ("B", "S", "M", "cu", "pos", "fp8", "mxfp4")
 
-    def __init__(self, B, S, M, cu, pos, fp8=False):
-        self.B, self.S, self.M, self.cu, self.pos, self.fp8 = B, S, M, cu, pos, fp8
+    def __init__(self, B, S, M, cu, pos, fp8=False, mxfp4=False):
+        self.B, self.S, self.M, self.cu, self.pos, self.fp8, self.mxfp4 = B, S, M, cu, pos, fp8, mxfp4
 
 
 class LlamaStack:
@@ -107,9 +107,11 @@ class LlamaStack:
 
     # -- parameters -----------------------------------------------------------------------------
     def invalidate_fp8(self) -> None:
-        """Drops the e4m3 copies of the weights (and the decode graphs captured on them): they are made lazily from the bf16
-        weights at the first fp8 call, so call this whenever the bf16 weights change (loading a checkpoint, a training step)."""
+        """Drops the e4m3 and MXFP4 copies of the weights (and the decode graphs captured on them): they are made lazily from the
+        bf16 weights at the first fp8 / mxfp4 call, so call this whenever the bf16 weights change (loading a checkpoint, a
+        training step)."""
         self._fp8_rw = None
+        self._mxfp4_w = None
         self.__dict__.pop("_dec_graphs_b", None)
 
     def init_random(self, seed: int = 0, std: float = 0.02):
@@ -160,10 +162,21 @@ class LlamaStack:
         return self._pos_cache[key]
 
     # -- forward --------------------------------------------------------------------------------
-    def new_cache(self, max_len: Optional[int] = None, batch: Optional[int] = None) -> List[torch.Tensor]:
+    def new_cache(self, max_len: Optional[int] = None, batch: Optional[int] = None, kv4: bool = False) -> list:
         """Per-layer [max_len, 3D] buffers in the fused qkv layout (k at column D, v at 2D); with `batch`: [B, max_len, 3D]
-        (lock-step generation of B samples)."""
+        (lock-step generation of B samples).  kv4 (with `batch`): one ops.KV4Cache per layer instead, keys and values in MXFP4 —
+        1.06 bytes per position and feature of D against the 6 of the bf16 buffer (which holds q's columns too)."""
         n = max_len or self.cfg.max_position_embeddings
+        if kv4:
+            assert batch is not None, "the 4-bit cache belongs to the lock-step decode (batch=...)"
+            kept = getattr(self, "_kv4_cache_b", None)
+            if kept is None or kept[0].k.shape[0] != batch or kept[0].k.shape[2] < n:
+                kept = None
+                self._kv4_cache_b = None                    # (as below: the old cache and the graphs captured on it go first)
+                self.__dict__.pop("_dec_graphs_b", None)
+                kept = [ops.KV4Cache.empty(batch, n, self.H, self.dh, self.device) for _ in range(self.L)]
+                self._kv4_cache_b = kept
+            return kept
         if batch is not None:
             kept = getattr(self, "_kv_cache_b", None)
             if kept is None or kept[0].shape[0] != batch or kept[0].shape[1] < n:
@@ -256,8 +269,7 @@ class LlamaStack:
         only and the output is [n, D]: the other rows' outputs of the last layer feed nothing (see forward(last_rows=...))."""
         lp = self.layers[li]
         eps, scale = self.cfg.rms_norm_eps, self.dh ** -0.5
-        mm = (lambda a, k, residual=None: self._mm_fp8(li, k, a, residual)) if seq.fp8 else \
-             (lambda a, k, residual=None: ops.gemm_nt(a, lp.w[k], residual=residual))
+        mm = self._layer_mm(li, seq.fp8, seq.mxfp4)
         probe = getattr(self, "_fp8_probe", None)
         # fp8 inference: RMSNorm writes the e4m3 rows + scales of the next GEMM itself (no bf16 copy, no quantise pass)
         fuse8 = seq.fp8 and not save and probe is None and self.D in (2048, 4096, 5120) and _FP8_FUSED_NORM
@@ -270,7 +282,10 @@ class LlamaStack:
         qkv = mm(xn, "qkv")
         ops.rope_qk_(qkv, self.cos, self.sin, seq.pos, self.H, self.dh)
         if cache is not None:
-            if cache[li].dim() == 2:                       # batch-1 cache [max_len, 3D] (native decode step)
+            if isinstance(cache[li], ops.KV4Cache):
+                assert seq.cu is None, "the 4-bit cache is filled from a padded batch"
+                ops.kv4_append(qkv, cache[li], None, self.H)
+            elif cache[li].dim() == 2:                       # batch-1 cache [max_len, 3D] (native decode step)
                 assert seq.B == 1
                 cache[li][:seq.S].copy_(qkv)
             else:                                          # batched cache [B, max_len, 3D]: only the k | v columns are ever read
@@ -309,7 +324,7 @@ class LlamaStack:
     def forward(self, x: torch.Tensor, B: int, S: int, save: Optional[bool] = None,
                 all_hidden: bool = False, cache: Optional[List[torch.Tensor]] = None,
                 cu_seqlens: Optional[torch.Tensor] = None, pos: Optional[torch.Tensor] = None, fp8: bool = False,
-                last_rows: Optional[torch.Tensor] = None):
+                last_rows: Optional[torch.Tensor] = None, mxfp4: bool = False):
         """x [M, D] bf16 -> final-normed hidden [M, D]  ([n, D] with last_rows, see below).
         Padded batch: M = B*S, sample b owns rows [b*S, (b+1)*S), positions arange(S) (right padding is harmless under the
         causal mask).  Packed batch (cu_seqlens int32 [B+1] on the device + pos int32 [M]): the B samples are stored end
@@ -327,9 +342,12 @@ class LlamaStack:
         assert (cu_seqlens is None and M == B * S) or (cu_seqlens is not None and pos is not None and pos.numel() == M)
         assert not (fp8 and save), "the fp8 GEMMs are an inference path (BASELINE config 5)"
         assert last_rows is None or (save and not all_hidden and cache is None), "last_rows: training passes without all_hidden"
+        assert not (mxfp4 and (save or fp8)), "the MXFP4 GEMMs are an inference path of their own"
         if fp8 and getattr(self, "_fp8_rw", None) is None:
             self.fp8_prepare_rowwise()
-        seq = SeqInfo(B=B, S=S, M=M, cu=cu_seqlens, pos=self._positions(B, S) if pos is None else pos, fp8=fp8)
+        if mxfp4 and getattr(self, "_mxfp4_w", None) is None:
+            self.mxfp4_prepare()
+        seq = SeqInfo(B=B, S=S, M=M, cu=cu_seqlens, pos=self._positions(B, S) if pos is None else pos, fp8=fp8, mxfp4=mxfp4)
         self.saved = []
         hs = [x] if all_hidden else None
         for li in range(self.L):
@@ -367,9 +385,33 @@ class LlamaStack:
         a8, inv_a = a if isinstance(a, tuple) else ops.quantize_fp8_rowwise(a)     # RMSNorm hands over e4m3 rows directly
         return ops.gemm_fp8_nt_scaled(a8, w8, inv_a, inv_w, residual=residual)
 
-    def decode_step_batched(self, x1: torch.Tensor, lens: torch.Tensor, cache: List[torch.Tensor], fp8: bool = False) -> torch.Tensor:
+    # -- MXFP4 GEMMs: 4-bit weights and activations, one power-of-two scale per 32 elements of K ---------------------------
+    def mxfp4_prepare(self) -> None:
+        """MXFP4 copies of the four GEMM weights of every layer (17/32 bytes per element; the bf16 weights stay, the copies are made
+        anew whenever those change: invalidate_fp8)."""
+        with torch.no_grad():
+            self.__dict__.pop("_dec_graphs_b", None)        # a captured decode step points at the old copies
+            self._mxfp4_w = [{k: ops.quantize_mxfp4(lp.w[k]) for k in ("qkv", "o", "gu", "down")} for lp in self.layers]
+
+    def _mm_mxfp4(self, li: int, key: str, a: torch.Tensor, residual=None) -> torch.Tensor:
+        w4 = self._mxfp4_w[li][key]
+        if a.shape[0] <= 32:        # decode steps: the cost is reading W once, the activations stay bf16 (no rounding of them)
+            return ops.gemm_w4a16_nt(a, w4, residual=residual)
+        return ops.gemm_mxfp4_nt(ops.quantize_mxfp4(a), w4, residual=residual)
+
+    def _layer_mm(self, li: int, fp8: bool, mxfp4: bool):
+        """mm(a, key, residual) = a @ W_key^T (+ residual) of layer li in the weight format asked for."""
+        if mxfp4:
+            return lambda a, k, residual=None: self._mm_mxfp4(li, k, a, residual)
+        if fp8:
+            return lambda a, k, residual=None: self._mm_fp8(li, k, a, residual)
+        w = self.layers[li].w
+        return lambda a, k, residual=None: ops.gemm_nt(a, w[k], residual=residual)
+
+    def decode_step_batched(self, x1: torch.Tensor, lens: torch.Tensor, cache: list, fp8: bool = False, mxfp4: bool = False) -> torch.Tensor:
         """One new token for each of B samples in lock step: x1 [B, D], lens int32 [B] (device) = position of the new token
-        of every sample = its current cache length; cache[l] [B, max_len, 3D].  Returns the final-normed hidden [B, D]
+        of every sample = its current cache length; cache[l] [B, max_len, 3D] or an ops.KV4Cache (new_cache(kv4=True)); the four
+        projections in bf16, e4m3 (fp8) or MXFP4 (mxfp4) weights, in any combination with the cache.  Returns the final-normed hidden [B, D]
         (valid until the next call).  Weights are streamed once per step for all B samples (GEMMs at M = B).
 
         The step is ~450 short launches (5 - 80 us each) and the generation loop needs its result on the host before it can
@@ -377,12 +419,18 @@ class LlamaStack:
         against 5 - 6 ms of kernels): the launch sequence is captured ONCE per (batch, cache, weight format) in a hipGraph —
         positions and lengths are device tensors, nothing in it depends on the token index — and replayed per token.
         HVLM_DECODE_BATCH_GRAPH=0 issues it eagerly (bit-identical, tests/test_gpu_fp8.py)."""
+        assert not (fp8 and mxfp4), "decode weights are e4m3 or MXFP4, not both"
         if fp8 and getattr(self, "_fp8_rw", None) is None:
             self.fp8_prepare_rowwise()                  # fp8_decode without an fp8 prefill: the e4m3 copies are made here
+        if mxfp4 and getattr(self, "_mxfp4_w", None) is None:
+            self.mxfp4_prepare()
         if os.environ.get("HVLM_DECODE_BATCH_GRAPH", "1") != "1" or not x1.is_cuda:
-            return self._decode_step_batched_eager(x1, lens, cache, fp8)
-        wkey = self._fp8_rw[0]["qkv"][0].data_ptr() if fp8 else self.layers[0].w["qkv"].data_ptr()
-        key = (x1.shape[0], bool(fp8), cache[0].data_ptr(), cache[0].shape[1], wkey)       # the graph holds raw pointers
+            return self._decode_step_batched_eager(x1, lens, cache, fp8, mxfp4)
+        wkey = (self._mxfp4_w[0]["qkv"][0] if mxfp4 else self._fp8_rw[0]["qkv"][0] if fp8 else self.layers[0].w["qkv"]).data_ptr()
+        if isinstance(cache[0], ops.KV4Cache):          # the graph holds raw pointers
+            key = (x1.shape[0], bool(fp8), bool(mxfp4), wkey, cache[0].k.shape[2]) + tuple(t.data_ptr() for c in cache for t in c)
+        else:
+            key = (x1.shape[0], bool(fp8), bool(mxfp4), wkey, cache[0].shape[1], cache[0].data_ptr())
         graphs = self.__dict__.setdefault("_dec_graphs_b", {})
         st = graphs.get(key)
         if st is None:
@@ -399,24 +447,27 @@ class LlamaStack:
                 side = torch.cuda.Stream(device=x1.device)
                 side.wait_stream(cur)
                 with torch.cuda.stream(side):           # warm-up outside the capture: lazy one-time initialisation in the library
-                    self._decode_step_batched_eager(sx, sl, cache, fp8)
+                    self._decode_step_batched_eager(sx, sl, cache, fp8, mxfp4)
                 cur.wait_stream(side)
                 g = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(g):
-                    out = self._decode_step_batched_eager(sx, sl, cache, fp8)
+                    out = self._decode_step_batched_eager(sx, sl, cache, fp8, mxfp4)
             finally:
                 ops.set_gemm_hook(hook)
-            st = (g, sx, sl, out)
+            st = (g, sx, sl, out, cache if isinstance(cache[0], ops.KV4Cache) else None)     # (a 4-bit cache lives as long as its graph)
             graphs[key] = st
-        g, sx, sl, out = st
+        g, sx, sl, out, _ = st
         sx.copy_(x1)
         sl.copy_(lens)
         g.replay()
         return out
 
-    def _decode_step_batched_eager(self, x1: torch.Tensor, lens: torch.Tensor, cache: List[torch.Tensor], fp8: bool = False) -> torch.Tensor:
+    def _decode_step_batched_eager(self, x1: torch.Tensor, lens: torch.Tensor, cache: list, fp8: bool = False, mxfp4: bool = False) -> torch.Tensor:
         if fp8 and getattr(self, "_fp8_rw", None) is None:
             self.fp8_prepare_rowwise()
+        if mxfp4 and getattr(self, "_mxfp4_w", None) is None:
+            self.mxfp4_prepare()
+        kv4 = isinstance(cache[0], ops.KV4Cache)
         B = x1.shape[0]
         eps, scale = self.cfg.rms_norm_eps, self.dh ** -0.5
         rows = torch.arange(B, device=self.device)
@@ -426,19 +477,22 @@ class LlamaStack:
         # q|k|v and gate|up: RoPE + cache row write / SwiGLU ride in the split-K finalize pass of the weight-streaming GEMM
         # (bit-identical, three launches fewer per layer); HVLM_DECODE_FUSED_FINALIZE=0 keeps them as separate kernels
         fused = (_DECODE_FUSED_FINALIZE and ops._GEMM_SKINNY and x1.is_cuda and B <= 32 and self.D % 64 == 0 and self.F % 4 == 0
-                 and self.D >= 256 and self.dh % 8 == 0)
+                 and self.D >= 256 and self.dh % 8 == 0 and not mxfp4)
         for li, lp in enumerate(self.layers):
-            mm = (lambda a, k, residual=None: self._mm_fp8(li, k, a, residual)) if fp8 else \
-                 (lambda a, k, residual=None: ops.gemm_nt(a, lp.w[k], residual=residual))
+            mm = self._layer_mm(li, fp8, mxfp4)
             wsel = (lambda k: self._fp8_rw[li][k]) if fp8 else (lambda k: lp.w[k])
             xn, _ = ops.rmsnorm_fwd(x, lp.w["ln1"], eps, save_rstd=False)
-            if fused:
+            if fused and not kv4:
                 qkv = ops.gemm_skinny_qkv(xn, wsel("qkv"), cache[li], lens, self.cos, self.sin, self.H, self.dh)
             else:
                 qkv = mm(xn, "qkv")
                 ops.rope_qk_(qkv, self.cos, self.sin, lens, self.H, self.dh)
-                cache[li][rows, idx] = qkv                               # the new token's k / v row of every sample
-            ao = ops.attn_decode_batched(qkv, cache[li], lens1, self.H, self.dh, scale)
+                if kv4:
+                    ops.kv4_append(qkv, cache[li], lens, self.H)
+                else:
+                    cache[li][rows, idx] = qkv                           # the new token's k / v row of every sample
+            ao = ops.attn_decode_kv4(qkv, cache[li], lens1, self.H, scale) if kv4 else \
+                ops.attn_decode_batched(qkv, cache[li], lens1, self.H, self.dh, scale)
             h = mm(ao, "o", residual=x)
             hn, _ = ops.rmsnorm_fwd(h, lp.w["ln2"], eps, save_rstd=False)
             act = ops.gemm_skinny_swiglu(hn, wsel("gu")) if fused else ops.swiglu_fwd(mm(hn, "gu"))

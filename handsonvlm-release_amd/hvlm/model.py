@@ -767,18 +767,22 @@ class HandsOnVLMForCausalLM:
     @torch.no_grad()
     def sample_batch(self, input_ids, logits_processor=None, max_length=None, eos_token_id=None, pad_token_id=None,
                      attention_mask=None, image=None, hand_noise=None, fp8: bool = False, fp8_decode: bool = False,
-                     fp8_clip: bool = False, output_scores: bool = False):
+                     fp8_clip: bool = False, output_scores: bool = False, mxfp4: bool = False, mxfp4_decode: bool = False,
+                     kv4: bool = False):
         """Lock-step generation of B samples (batch-32 evaluation).  The reference's sample() is batch 1
         (`.item()` at handsonvlm.py:609) and re-runs CLIP + the whole prefix per token; this is the same per-sample function
         — multinomial sampling, a CVAE hand decoded from the last hidden state whenever token 32100 is drawn, that hand's
         sinusoidal encoding added to the token's embedding when it is fed back (handsonvlm.py:380-396,543-647) — with one
         batched prefill (bf16, or the e4m3 GEMMs with `fp8`) filling a [B, max_len, 3D] KV cache per layer and one batched
         decode step per generated token (weights streamed once for all B samples; e4m3 weights with `fp8_decode`).
-        `fp8_clip` runs the CLIP tower's layer GEMMs on e4m3 operands as well.  Right-padded prompts (attention_mask)
+        `fp8_clip` runs the CLIP tower's layer GEMMs on e4m3 operands as well.  `mxfp4` / `mxfp4_decode`: the same two places in
+        MXFP4 (4-bit weights and activations in the prefill, 4-bit weights in the decode steps); `kv4`: keys and values are kept in
+        MXFP4 (a quarter of their bytes; the prefill itself attends to the unrounded ones).  Right-padded prompts (attention_mask)
         are supported: a sample's pad rows are never attended (its own length bounds its keys).
         `logits_processor`: callables (input_ids [B, cur], scores [B, V]) -> scores.  `hand_noise[b][j]`: optional z for the
         j-th hand of sample b.  Returns SampleDecoderOnlyOutput(sequences [B, T_max] padded with pad_token_id,
         pred_hands [B, 2, n_max, 2] zero-padded) plus `.lengths` / `.num_hands` lists."""
+        assert not (fp8 and mxfp4) and not (fp8_decode and mxfp4_decode), "prefill and decode weights are e4m3 or MXFP4, not both"
         cfg, dev = self.config, self.device
         B, T = input_ids.shape
         procs = list(logits_processor or [])
@@ -798,9 +802,9 @@ class HandsOnVLMForCausalLM:
         lengths = plan.lengths - npad
         n_gen = 160 if max_length is None else max(1, max_length - T)
         max_len = min(cfg.max_position_embeddings, S + n_gen)
-        cache = self.stack.new_cache(max_len, batch=B)
+        cache = self.stack.new_cache(max_len, batch=B, kv4=kv4)
         x = ops.embed_splice_fwd(self.embed, vis, plan.src, None, None, None, B, S, self.token_dim, NV, 1)
-        hidden = self.stack.forward(x, B, S, save=False, cache=cache, fp8=fp8)
+        hidden = self.stack.forward(x, B, S, save=False, cache=cache, fp8=fp8, mxfp4=mxfp4)
         rows = torch.from_numpy((np.arange(B) * S + lengths - 1).astype(np.int64)).to(dev)
         last = hidden[rows].contiguous()                                        # [B, D]
         del hidden, x
@@ -848,7 +852,7 @@ class HandsOnVLMForCausalLM:
             x1 = ops.embed_splice_fwd(self.embed, None, src, slot, hand_new.contiguous(), torch.ones(B, device=dev), B, 1,
                                       self.token_dim, 0, 1)
             # (finished samples stay at their last row: their writes must not run past the cache)
-            last = self.stack.decode_step_batched(x1, lens, cache, fp8=fp8_decode)
+            last = self.stack.decode_step_batched(x1, lens, cache, fp8=fp8_decode, mxfp4=mxfp4_decode)
             lens_h[~done] += 1
             lens = lens + torch.from_numpy((~done).astype(np.int32)).to(dev)
         tmax = max(len(q) for q in seqs)
