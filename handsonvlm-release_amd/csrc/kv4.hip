@@ -14,16 +14,21 @@
 // The codes of a tile (K 2 KB, V 2 KB) come by LDS-DMA, 1 KB of consecutive rows an instruction, into a ring of the wave's own, three tiles ahead
 // and without a barrier; loaded into registers in fragment order a tile would take 20 instructions instead of 6 and the address units
 // would bound the kernel.  A tile's scales are two more.
-// Softmax: running maximum and sum per wave in fp32; P is rounded to bf16 for the second product (its error, 2^-9 relative and
+// Softmax: running maximum and sum per wave in fp32; P is rounded to bf16 for the second product (its error, at most 2^-8 relative and
 // independent from key to key, is below that of the bf16 result).  The waves of a workgroup take alternate tiles and merge in LDS; the
 // workgroups of a split sample write (max, sum, unnormalised row) in fp32 and a second kernel joins them in order: no atomics.
 // Rows at and past lens[b] are never read.
+//
+// Bound by the read of the cache when there are many keys: 32 samples x 32 heads, 98 MB, 28 - 30 us; 8 samples x 8 KV
+// heads of up to 32768 keys, 214 MB, 40 - 49 us and 4.7 us to join (from HBM at the rate of a copy, 4.79 TB/s, these take 20 and 45 us; what earlier
+// calls left in the last-level cache comes faster).  Short caches by latency: one sample x 32 heads x 1024 keys 9 us.
 #include "mxfp4.h"
 
 namespace hvlm {
 namespace {
 
-constexpr int KV4_WAVES = 4;
+constexpr int KV4_WAVES = 4;                // of a workgroup of the attention
+constexpr int KV4_WIDE = 8;                 // of its form for short caches
 constexpr int KV4_TILE = 32;               // keys per wave and step
 
 // ---- append -----------------------------------------------------------------------------------------------------------------------
@@ -81,7 +86,7 @@ __device__ __forceinline__ void kv4_wait() {                                  //
 }
 
 // (a __device__ template under plain __global__ wrappers, as in gemm_pp.hip)
-template <int DH>
+template <int DH, int WAVES>
 __device__ __forceinline__ void attn_decode_kv4_body(const Kv4Args& p) {
   constexpr int KD = DH / 4;              // dims of a key per lane: KD / 2 bytes
   constexpr int VD = DH / 16;             // dims of a value row per lane: VD / 2 bytes
@@ -94,7 +99,7 @@ __device__ __forceinline__ void attn_decode_kv4_body(const Kv4Args& p) {
   const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const long len = min((long)max(p.lens[b], 0), p.max_len);
   // keys of this split: a whole number of rounds of the workgroup
-  const long round = KV4_WAVES * KV4_TILE;
+  const long round = WAVES * KV4_TILE;
   const long per = ((len + p.splits - 1) / p.splits + round - 1) / round * round;
   const long k0 = min(per * split, len), k1 = min(k0 + per, len);
   const long base = (long)bh * p.max_len;
@@ -229,8 +234,8 @@ __device__ __forceinline__ void attn_decode_kv4_body(const Kv4Args& p) {
   __syncthreads();                                                             // the rings become the rows to merge
 
   // merge: lane holds dims (4 g + i) VD + j of head r16
-  float* sm_m = sm + KV4_WAVES * p.G * DH;
-  float* sm_l = sm_m + KV4_WAVES * p.G;
+  float* sm_m = sm + WAVES * p.G * DH;
+  float* sm_l = sm_m + WAVES * p.G;
   if (r16 < p.G) {
     float* row = sm + (w * p.G + r16) * DH + 4 * g * VD;
 #pragma unroll
@@ -240,15 +245,15 @@ __device__ __forceinline__ void attn_decode_kv4_body(const Kv4Args& p) {
     if (g == 0) { sm_m[w * p.G + r16] = mx; sm_l[w * p.G + r16] = sum; }
   }
   __syncthreads();
-  for (int i = t; i < p.G * DH; i += KV4_WAVES * 64) {
+  for (int i = t; i < p.G * DH; i += WAVES * 64) {
     const int h = i / DH, d = i - h * DH;
     float m = sm_m[h];
 #pragma unroll
-    for (int v = 1; v < KV4_WAVES; ++v) m = fmaxf(m, sm_m[v * p.G + h]);
+    for (int v = 1; v < WAVES; ++v) m = fmaxf(m, sm_m[v * p.G + h]);
     const float off = m == -INFINITY ? 0.f : m;
     float acc = 0.f, den = 0.f;
 #pragma unroll
-    for (int v = 0; v < KV4_WAVES; ++v) {
+    for (int v = 0; v < WAVES; ++v) {
       const float f = __builtin_amdgcn_exp2f(sm_m[v * p.G + h] - off);
       acc += f * sm[(v * p.G + h) * DH + d];
       den += f * sm_l[v * p.G + h];
@@ -264,8 +269,10 @@ __device__ __forceinline__ void attn_decode_kv4_body(const Kv4Args& p) {
   }
 }
 
-__global__ __launch_bounds__(KV4_WAVES * 64, 2) void attn_decode_kv4_128_kernel(Kv4Args p) { attn_decode_kv4_body<128>(p); }
-__global__ __launch_bounds__(KV4_WAVES * 64, 2) void attn_decode_kv4_64_kernel(Kv4Args p) { attn_decode_kv4_body<64>(p); }
+__global__ __launch_bounds__(KV4_WAVES * 64, 2) void attn_decode_kv4_128_kernel(Kv4Args p) { attn_decode_kv4_body<128, KV4_WAVES>(p); }
+__global__ __launch_bounds__(KV4_WAVES * 64, 2) void attn_decode_kv4_64_kernel(Kv4Args p) { attn_decode_kv4_body<64, KV4_WAVES>(p); }
+__global__ __launch_bounds__(KV4_WIDE * 64, 2) void attn_decode_kv4_128_wide_kernel(Kv4Args p) { attn_decode_kv4_body<128, KV4_WIDE>(p); }
+__global__ __launch_bounds__(KV4_WIDE * 64, 2) void attn_decode_kv4_64_wide_kernel(Kv4Args p) { attn_decode_kv4_body<64, KV4_WIDE>(p); }
 
 // Joins the splits of one head: KV4_JOIN groups of DH threads take every KV4_JOIN-th split, all of a group's loads at once up to eight, and merge
 // in LDS, in order.
@@ -318,12 +325,20 @@ __global__ __launch_bounds__(KV4_JOIN * DH) void kv4_combine_kernel(const float*
   out[(head / H) * ldo + (head % H) * DH + d] = f2bf(den == 0.f ? 0.f : acc / den);
 }
 
-// splits of the key axis: enough workgroups for four on every CU (two: 49 us against 41 us at one sequence of 32768 keys, 32 heads), but no split shorter than one round of a workgroup
-int kv4_splits(int B, int Hkv, long max_len) {
+// Splits of the key axis, waves of a workgroup.  Long caches and few heads: enough workgroups for four on every CU (with two, 49 us against
+// 41 us at 8 samples x 8 KV heads of up to 32768 keys), but no split shorter than one round of a workgroup, and a second kernel that joins.
+// Short caches whose workgroups have a CU each: one of eight waves reads all of a head's keys and nothing is joined.  Measured (us, one against
+// two kernels, dh = 128): 32 heads x 256 keys 4.9 / 6.3, x 1024 9.2 / 8.0 (and one launch of the host less), x 2048 13.7 / 9.6; 128 x 2048 15.9 / 18.2,
+// x 4096 25.7 / 24.4; 256 x 4096 32.5 / 38.3; 520 heads x 1024, two or three to a CU, 31.5 / 26.8.
+struct Kv4Plan {
+  int waves, splits;
+};
+Kv4Plan kv4_plan(int B, int Hkv, long max_len) {
   const long pairs = (long)B * Hkv, rounds = (max_len + KV4_WAVES * KV4_TILE - 1) / (KV4_WAVES * KV4_TILE);
   long s = (1024 + pairs - 1) / pairs;
   if (s > rounds) s = rounds;
-  return (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+  if (s > 1 && pairs <= 256 && max_len <= (pairs > 64 ? 16 * pairs : 1024)) return {KV4_WIDE, 1};
+  return {KV4_WAVES, (int)(s < 1 ? 1 : s > 256 ? 256 : s)};
 }
 
 }  // namespace
@@ -355,7 +370,7 @@ extern "C" int hvlm_kv4_append(const void* qkv, long ld, void* k_codes, void* k_
 
 extern "C" size_t hvlm_attn_decode_kv4_ws_bytes(int B, int H, int Hkv, int dh, long max_len) {
   if (B <= 0 || H <= 0 || Hkv <= 0 || dh <= 0 || max_len <= 0) return 0;
-  const int s = kv4_splits(B, Hkv, max_len);
+  const int s = kv4_plan(B, Hkv, max_len).splits;
   return s == 1 ? 0 : (size_t)B * H * s * (dh + 2) * 4;
 }
 
@@ -368,18 +383,24 @@ extern "C" int hvlm_attn_decode_kv4(const void* q, long ldq, const void* k_codes
   HVLM_REQUIRE(H % Hkv == 0 && H / Hkv <= 16, "attn_decode_kv4: H=%d must be 1 to 16 times Hkv=%d", H, Hkv);
   HVLM_REQUIRE(ldq >= (long)H * dh && ldq % 8 == 0 && ((uintptr_t)q & 15) == 0, "attn_decode_kv4: rows of q must be 16-byte aligned");
   HVLM_REQUIRE(ldo >= (long)H * dh, "attn_decode_kv4: leading dimension of out");
-  const int splits = kv4_splits(B, Hkv, max_len), G = H / Hkv;
+  const Kv4Plan plan = kv4_plan(B, Hkv, max_len);
+  const int splits = plan.splits, waves = plan.waves, G = H / Hkv;
   HVLM_REQUIRE(splits == 1 || (ws && ((uintptr_t)ws & 15) == 0), "attn_decode_kv4: a 16-byte aligned workspace of hvlm_attn_decode_kv4_ws_bytes() is needed");
   Kv4Args p{};
   p.q = (const bf16_t*)q; p.kc = (const unsigned char*)k_codes; p.ks = (const unsigned char*)k_scales; p.vc = (const unsigned char*)v_codes;
   p.vs = (const unsigned char*)v_scales; p.lens = lens; p.out = (bf16_t*)out; p.ws = (float*)ws; p.ldq = ldq; p.ldo = ldo; p.max_len = max_len;
   p.H = H; p.Hkv = Hkv; p.G = G; p.splits = splits; p.scale_log2 = scale * 1.4426950408889634f;
-  const size_t merge = (size_t)KV4_WAVES * G * (dh + 2) * 4, rings = (size_t)KV4_WAVES * KV4_RING * (KV4_TILE * dh + 512);
-  const size_t lds = merge > rings ? merge : rings;                           // 72 KB at dh = 128, 40 KB at dh = 64
-  const auto k = dh == 128 ? attn_decode_kv4_128_kernel : attn_decode_kv4_64_kernel;
-  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_decode_kv4_128_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 73728);
-  if (attr != hipSuccess) { set_error("attn_decode_kv4: hipFuncSetAttribute: %s", hipGetErrorString(attr)); return HVLM_ERR_LAUNCH; }
-  hipLaunchKernelGGL(k, dim3((unsigned)(B * Hkv * splits)), dim3(KV4_WAVES * 64), lds, as_stream(stream), p);
+  const size_t merge = (size_t)waves * G * (dh + 2) * 4, rings = (size_t)waves * KV4_RING * (KV4_TILE * dh + 512);
+  const size_t lds = merge > rings ? merge : rings;                           // a wave's ring is 18 KB at dh = 128, 10 KB at dh = 64
+  const auto k = dh == 128 ? (waves == KV4_WIDE ? attn_decode_kv4_128_wide_kernel : attn_decode_kv4_128_kernel)
+                           : (waves == KV4_WIDE ? attn_decode_kv4_64_wide_kernel : attn_decode_kv4_64_kernel);
+  const auto set = [](void (*f)(Kv4Args), int bytes) { return hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, bytes); };
+  static const hipError_t a1 = set(attn_decode_kv4_128_kernel, 73728), a2 = set(attn_decode_kv4_128_wide_kernel, 147456), a3 = set(attn_decode_kv4_64_wide_kernel, 81920);
+  if (a1 != hipSuccess || a2 != hipSuccess || a3 != hipSuccess) {
+    set_error("attn_decode_kv4: hipFuncSetAttribute: %s", hipGetErrorString(a1 != hipSuccess ? a1 : a2 != hipSuccess ? a2 : a3));
+    return HVLM_ERR_LAUNCH;
+  }
+  hipLaunchKernelGGL(k, dim3((unsigned)(B * Hkv * splits)), dim3((unsigned)waves * 64), lds, as_stream(stream), p);
   const int rc2 = check_launch("attn_decode_kv4");
   if (rc2 || splits == 1) return rc2;
   const auto c = dh == 128 ? kv4_combine_kernel<128> : kv4_combine_kernel<64>;

@@ -515,7 +515,7 @@ int hvlm_gemm_mxfp4_nt(const void* A, const void* a_scale, const void* B, const 
                        long ldas, long ldb, long ldbs, long ldc, const void* bias, const void* residual, long ldr, int act, int out_f32,
                        void* ws, void* stream);
 /* The weight-streaming form for M <= 32 (decode steps): x [M, K] in bf16 against MXFP4 weights, C in bf16.  ws: 16-byte aligned,
- * hvlm_gemm_w4a16_ws_bytes(M, N, K) bytes, not initialised, used until the call's work on `stream` is done. */
+ * hvlm_gemm_w4a16_ws_bytes(M, N, K) bytes (0: may be NULL), not initialised, used until the call's work on `stream` is done. */
 size_t hvlm_gemm_w4a16_ws_bytes(int M, int N, int K);
 int hvlm_gemm_w4a16_nt(const void* x, const void* W, const void* w_scale, void* C, int M, int N, int K, long ldx, long ldw, long ldws,
                        long ldc, const void* bias, const void* residual, long ldr, int act, void* ws, void* stream);
@@ -525,7 +525,7 @@ int hvlm_gemm_w4a16_nt(const void* x, const void* W, const void* w_scale, void* 
  *       start (NULL: 0) and count (NULL: S; rows s >= count[b] are skipped) are device int32 [B]; rows outside the cache are dropped.
  *   attn_decode: out[b, h] = softmax(scale * q[b, h] . K)[t < lens[b]] V for one query row per sample; head h reads KV head
  *       h / (H / Hkv), H / Hkv <= 16.  lens: device int32 [B], clamped to 0 .. max_len; a sample of length 0 gives zeros.  Cache rows at and
- *       past lens[b] are never used, whatever they hold.  ws: as above, hvlm_attn_decode_kv4_ws_bytes() bytes (0: may be NULL). */
+ *       past lens[b] are never read.  ws: as above, hvlm_attn_decode_kv4_ws_bytes() bytes (0: may be NULL). */
 int hvlm_kv4_append(const void* qkv, long ld, void* k_codes, void* k_scales, void* v_codes, void* v_scales, const int32_t* start,
                     const int32_t* count, int B, int S, long max_len, int H, int Hkv, int dh, void* stream);
 size_t hvlm_attn_decode_kv4_ws_bytes(int B, int H, int Hkv, int dh, long max_len);

@@ -117,12 +117,14 @@ def test_c_refusals(ops):
     bad(gm(ws=odd), "workspace")
     assert lib.hvlm_gemm_mxfp4_ws_bytes(0, 4, 32) == 0 and lib.hvlm_gemm_mxfp4_ws_bytes(867, 4096, 4096) == (7 + 32) * 2 * 32 * 256
     sk = lambda M=1, K=32, ldx=32, ws=p, x=p: lib.hvlm_gemm_w4a16_nt(x, p, p, p, M, 4, K, ldx, 16 * (K // 32), K // 32, 4, N, N, 0, 0, ws, N)  # noqa: E731
-    bad(sk(ws=N), "null")
+    bad(sk(x=N), "null")
+    bad(sk(M=5, ws=N), "workspace")
+    bad(sk(K=16416, ldx=16416, ws=N), "workspace")
     bad(sk(M=33), "1 .. 32")
     bad(sk(M=0), "1 .. 32")
     bad(sk(K=40, ldx=40), "multiple of 32")
     bad(sk(x=odd), "16-byte")
-    bad(sk(ws=odd), "workspace")
+    bad(sk(M=5, ws=odd), "workspace")
     ap = lambda ld=192, B=1, S=1, n=4, H=1, dh=64, q=p, kc=p: lib.hvlm_kv4_append(q, ld, kc, p, p, p, N, N, B, S, n, H, 1, dh, N)  # noqa: E731
     bad(ap(q=N), "null")
     bad(ap(kc=N), "null")
@@ -140,6 +142,7 @@ def test_c_refusals(ops):
     bad(at(ldo=32), "out")
     bad(at(n=0), "positive")
     bad(at(n=100000, ws=N), "workspace")
-    assert lib.hvlm_attn_decode_kv4_ws_bytes(64, 32, 32, 128, 1000) == 0 and lib.hvlm_attn_decode_kv4_ws_bytes(1, 32, 32, 128, 1000) > 0
+    assert lib.hvlm_attn_decode_kv4_ws_bytes(64, 32, 32, 128, 1000) == 0 and lib.hvlm_attn_decode_kv4_ws_bytes(1, 32, 32, 128, 1000) == 0
+    assert lib.hvlm_attn_decode_kv4_ws_bytes(1, 32, 32, 128, 1025) == 32 * 9 * 130 * 4
     assert lib.hvlm_attn_decode_kv4_ws_bytes(0, 32, 32, 128, 1000) == 0 and lib.hvlm_gemm_w4a16_ws_bytes(0, 4, 32) == 0
-    assert lib.hvlm_gemm_w4a16_ws_bytes(3, 5, 32) == 3 * 8 * 4
+    assert lib.hvlm_gemm_w4a16_ws_bytes(4, 5, 4096) == 0 and lib.hvlm_gemm_w4a16_ws_bytes(1, 5, 16384) == 0 and lib.hvlm_gemm_w4a16_ws_bytes(5, 5, 32) == 5 * 8 * 4
