@@ -203,7 +203,7 @@ def test_gemm_past_32_bit_offsets(ops):
     check_product(ops.gemm_mxfp4_nt(a, b)[-50:], mx_ref.values((a[0][-50:], a[1][-50:])), mx_ref.values(b))
 
 
-SKINNY = list(itertools.product((1, 2, 7, 13, 16, 17, 32), ((1, 32), (130, 96), (515, 1056), (4096, 4096), (1000, 13824)))) + [(1, (22016, 4096)), (1, (48, 16384)), (1, (100, 16416)), (3, (33, 4128)), (2, (40, 8192)), (4, (40, 4096)), (4, (17, 160)), (32, (5120, 13824))]
+SKINNY = list(itertools.product((1, 2, 7, 13, 16, 17, 32), ((1, 32), (130, 96), (515, 1056), (4096, 4096), (1000, 13824)))) + [(1, (22016, 4096)), (1, (48, 14336)), (1, (100, 14368)), (2, (50, 7168)), (3, (50, 4768)), (3, (33, 4128)), (2, (40, 8192)), (4, (40, 4096)), (4, (17, 160)), (32, (5120, 13824))]
 
 
 @pytest.mark.parametrize("M,NK", SKINNY)

@@ -119,7 +119,7 @@ def test_c_refusals(ops):
     sk = lambda M=1, K=32, ldx=32, ws=p, x=p: lib.hvlm_gemm_w4a16_nt(x, p, p, p, M, 4, K, ldx, 16 * (K // 32), K // 32, 4, N, N, 0, 0, ws, N)  # noqa: E731
     bad(sk(x=N), "null")
     bad(sk(M=5, ws=N), "workspace")
-    bad(sk(K=16416, ldx=16416, ws=N), "workspace")
+    bad(sk(K=14368, ldx=14368, ws=N), "workspace")
     bad(sk(M=33), "1 .. 32")
     bad(sk(M=0), "1 .. 32")
     bad(sk(K=40, ldx=40), "multiple of 32")
@@ -145,4 +145,4 @@ def test_c_refusals(ops):
     assert lib.hvlm_attn_decode_kv4_ws_bytes(64, 32, 32, 128, 1000) == 0 and lib.hvlm_attn_decode_kv4_ws_bytes(1, 32, 32, 128, 1000) == 0
     assert lib.hvlm_attn_decode_kv4_ws_bytes(1, 32, 32, 128, 1025) == 32 * 9 * 130 * 4
     assert lib.hvlm_attn_decode_kv4_ws_bytes(0, 32, 32, 128, 1000) == 0 and lib.hvlm_gemm_w4a16_ws_bytes(0, 4, 32) == 0
-    assert lib.hvlm_gemm_w4a16_ws_bytes(4, 5, 4096) == 0 and lib.hvlm_gemm_w4a16_ws_bytes(1, 5, 16384) == 0 and lib.hvlm_gemm_w4a16_ws_bytes(5, 5, 32) == 5 * 8 * 4
+    assert lib.hvlm_gemm_w4a16_ws_bytes(4, 5, 4096) == 0 and lib.hvlm_gemm_w4a16_ws_bytes(1, 5, 14336) == 0 and lib.hvlm_gemm_w4a16_ws_bytes(5, 5, 32) == 5 * 8 * 4
