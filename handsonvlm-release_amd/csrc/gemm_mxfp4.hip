@@ -15,7 +15,7 @@
 //   * scales are tiled once per call by a kernel of their own (3 us at 22 016 rows of 4096) so that a step's fit one dword per four fragments:
 //     gathered row by row inside the K loop they cost a quarter of it (0.15 of 0.78 us a step);
 //   * workgroups are persistent and the ring runs on into the next tile, whose first 512 k land during the last of this one.
-// 13872 x 22016 x 4096: 610 us = 4.1 PFLOP/s (two groups of four waves one barrier apart, the shape of gemm_pp.hip: 723 us).  Without DMA and
+// 13872 x 22016 x 4096: 579 us = 4.3 PFLOP/s (two groups of four waves one barrier apart, the shape of gemm_pp.hip: 723 us).  Without DMA and
 // scales a step would take 0.46 us instead of 0.62, the products alone 0.43; the rest is the tiles' ends (vision shapes with K = 1024 are
 // mostly that: 90 us where the result's bytes need 44).
 #include "mxfp4.h"

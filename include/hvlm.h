@@ -514,7 +514,7 @@ size_t hvlm_gemm_mxfp4_ws_bytes(int M, int N, int K);
 int hvlm_gemm_mxfp4_nt(const void* A, const void* a_scale, const void* B, const void* b_scale, void* C, int M, int N, int K, long lda,
                        long ldas, long ldb, long ldbs, long ldc, const void* bias, const void* residual, long ldr, int act, int out_f32,
                        void* ws, void* stream);
-/* The weight-streaming form for M <= 32 (decode steps): x [M, K] in bf16 against MXFP4 weights, C in bf16.  ws: 16-byte aligned,
+/* The weight-streaming form for M <= 32 (decode steps): x [M, K] in bf16 against MXFP4 weights, C in bf16; residual may be C itself.  ws: 16-byte aligned,
  * hvlm_gemm_w4a16_ws_bytes(M, N, K) bytes (0: may be NULL), not initialised, used until the call's work on `stream` is done. */
 size_t hvlm_gemm_w4a16_ws_bytes(int M, int N, int K);
 int hvlm_gemm_w4a16_nt(const void* x, const void* W, const void* w_scale, void* C, int M, int N, int K, long ldx, long ldw, long ldws,

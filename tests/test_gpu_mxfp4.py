@@ -438,6 +438,20 @@ def test_step_against_definition_streams_and_graph(ops):
             same(a, b)
 
 
+@pytest.mark.parametrize("M,N,K", [(3, 515, 4096), (30, 130, 1056), (130, 333, 96), (600, 900, 512)])
+def test_the_result_may_take_the_residual_s_place(ops, M, N, K):
+    g = gen(13)
+    a, b = mx_ref.random_pair(M, K, g, "cuda"), mx_ref.random_pair(N, K, g, "cuda")
+    res = torch.randn(M, N, device="cuda", generator=g).to(BF16)
+    calls = [lambda r, out: ops.gemm_mxfp4_nt(a, b, residual=r, out=out)]
+    if M <= 32:
+        x = torch.randn(M, K, device="cuda", generator=g).to(BF16)
+        calls.append(lambda r, out: ops.gemm_w4a16_nt(x, b, residual=r, out=out))
+    for call in calls:
+        place = res.clone()
+        same(call(place, place), call(res, None))
+
+
 def test_results_do_not_depend_on_what_ran_before(ops):
     """The same call twice with other shapes between: the same bits (no state is kept, no atomics)."""
     g = gen(12)
