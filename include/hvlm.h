@@ -497,7 +497,7 @@ int hvlm_cast_bf16_to_f32(const void* in, float* out, long n, void* stream);
  *   codes  : 4-bit E2M1 {0, 0.5, 1, 1.5, 2, 3, 4, 6} with a sign bit, two per byte, the even element in the low nibble: K / 2 bytes a row
  *   scales : one E8M0 byte s per 32 elements, 2^(s - 127); 255 = the whole block is NaN: K / 32 bytes a row, at any alignment
  *   value  : code * 2^(s - 127)
- * Leading dimensions of codes and scales are in BYTES.  Every K is a multiple of 32.
+ * Leading dimensions of codes and scales are in BYTES.  Every K is a multiple of 32.  Outputs overlap no input, but where noted.
  * ------------------------------------------------------------------------------------------ */
 /* x [rows, K] (bf16, or IEEE half when f16 != 0; ldx elements) -> codes, scales: s - 127 = floor(log2(max |x|)) - 2 (at least -127),
  * elements round to nearest even and saturate at 6; a block that holds an infinity or a NaN becomes NaN.  Rows of x are 16-byte,
