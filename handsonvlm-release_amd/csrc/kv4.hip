@@ -352,6 +352,7 @@ static int kv4_check(const char* what, const void* kc, const void* ks, const voi
   HVLM_REQUIRE(dh == 64 || dh == 128, "%s: head dimension %d (64 or 128)", what, dh);
   HVLM_REQUIRE(max_len < (1L << 31) && (long)B * Hkv < (1L << 22), "%s: cache too large", what);
   HVLM_REQUIRE((((uintptr_t)kc | (uintptr_t)vc) & 15) == 0, "%s: codes must be 16-byte aligned", what);
+  HVLM_REQUIRE((((uintptr_t)ks | (uintptr_t)vs) & (dh / 32 - 1)) == 0, "%s: scales must be aligned to a row's %d bytes", what, dh / 32);
   return HVLM_OK;
 }
 

@@ -366,14 +366,13 @@ def _fail(msg: str):
 def _launch_stream(name: str, *tensors) -> int:
     """The current stream of the current device, on which every tensor has to be: a launch goes to that device, whatever the tensors say.
     (The raw handle: these calls are a few microseconds long, a Stream object would be a good part of them.)"""
-    dev = -1
+    dev = -2
     for t in tensors:
         if t is not None:
             d = t.get_device()
-            if dev < 0:
-                dev = d
-            if d < 0 or d != dev or d != torch._C._cuda_getDevice():
+            if d != dev and (d < 0 or dev >= 0 or d != torch._C._cuda_getDevice()):
                 _fail(f"{name}: expected tensors on the current device, got {t.device} (the HIP path has no CPU fallback)")
+            dev = d
     return torch._C._cuda_getCurrentRawStream(dev)
 
 

@@ -520,7 +520,7 @@ size_t hvlm_gemm_w4a16_ws_bytes(int M, int N, int K);
 int hvlm_gemm_w4a16_nt(const void* x, const void* W, const void* w_scale, void* C, int M, int N, int K, long ldx, long ldw, long ldws,
                        long ldc, const void* bias, const void* residual, long ldr, int act, void* ws, void* stream);
 /* KV cache in MXFP4, per K and V: codes [B, Hkv, max_len, dh / 2], scales [B, Hkv, max_len, dh / 32], dense (one head's rows are contiguous;
- * blocks run along the head dimension).  dh = 64 or 128; codes 16-byte aligned.
+ * blocks run along the head dimension).  dh = 64 or 128; codes 16-byte aligned, scales to dh / 32 bytes.
  *   append: row (b, s) of qkv [B * S, ld] (q | k | v columns: H, Hkv and Hkv heads; k after RoPE) -> cache row start[b] + s of sample b.
  *       start (NULL: 0) and count (NULL: S; rows s >= count[b] are skipped) are device int32 [B]; rows outside the cache are dropped.
  *   attn_decode: out[b, h] = softmax(scale * q[b, h] . K)[t < lens[b]] V for one query row per sample; head h reads KV head

@@ -142,6 +142,10 @@ def test_c_refusals(ops):
     bad(at(ldo=32), "out")
     bad(at(n=0), "positive")
     bad(at(n=100000, ws=N), "workspace")
+    for dh, off in ((128, 1), (128, 2), (64, 1)):                               # scales that a row's bytes straddle
+        s = ctypes.c_void_p((1 << 20) + off)
+        bad(lib.hvlm_kv4_append(p, 3 * dh, p, s, p, p, N, N, 1, 1, 4, 1, 1, dh, N), "scales must be aligned")
+        bad(lib.hvlm_attn_decode_kv4(p, dh, p, p, p, s, p, p, dh, 1, 4, 1, 1, dh, 0.1, p, N), "scales must be aligned")
     assert lib.hvlm_attn_decode_kv4_ws_bytes(64, 32, 32, 128, 1000) == 0 and lib.hvlm_attn_decode_kv4_ws_bytes(1, 32, 32, 128, 1000) == 0
     assert lib.hvlm_attn_decode_kv4_ws_bytes(1, 32, 32, 128, 1025) == 32 * 9 * 130 * 4
     assert lib.hvlm_attn_decode_kv4_ws_bytes(0, 32, 32, 128, 1000) == 0 and lib.hvlm_gemm_w4a16_ws_bytes(0, 4, 32) == 0
