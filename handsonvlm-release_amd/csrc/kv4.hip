@@ -325,20 +325,22 @@ __global__ __launch_bounds__(KV4_JOIN * DH) void kv4_combine_kernel(const float*
   out[(head / H) * ldo + (head % H) * DH + d] = f2bf(den == 0.f ? 0.f : acc / den);
 }
 
-// Splits of the key axis, waves of a workgroup.  Long caches and few heads: enough workgroups for four on every CU (with two, 49 us against
-// 41 us at 8 samples x 8 KV heads of up to 32768 keys), but no split shorter than one round of a workgroup, and a second kernel that joins.
-// Short caches whose workgroups have a CU each: one of eight waves reads all of a head's keys and nothing is joined.  Measured (us, one against
-// two kernels, dh = 128): 32 heads x 256 keys 4.9 / 6.3, x 1024 9.2 / 8.0 (and one launch of the host less), x 2048 13.7 / 9.6; 128 x 2048 15.9 / 18.2,
-// x 4096 25.7 / 24.4; 256 x 4096 32.5 / 38.3; 520 heads x 1024, two or three to a CU, 31.5 / 26.8.
+// Splits of the key axis, waves of a workgroup, by the number of (sample, KV head) pairs and the length of the cache.  Two workgroups fit a CU.
+//   Up to 256 pairs, short caches: a workgroup of eight waves reads all of a head's keys and nothing is joined.  Longer ones: one round of splits (512
+//   workgroups), joined by a second kernel; where samples may differ by many thousands of keys two rounds, so that the short ones make room.
+//   Beyond 256 pairs: no split, but for long caches, whose last round would be long.
+// Measured (us; all keys used, dh = 128): 32 pairs x 256 keys one kernel 4.9, two 6.4; x 1024 9.1 / 8.1 (and a launch of the host more);
+// x 8192 8, 16, 32 splits 16.2, 16.7, 20.1; 128 pairs x 2048 one kernel 16.1, two 15.6, x 4096 26.0 / 21.5; 64 pairs x 32768 8, 16 splits 60.6, 64.4, but 49 / 41
+// with lengths spread from 1000 to 32768; 520 pairs x 967 1, 2 splits 24.1, 26.5, x 4096 75.5, 68.2.
 struct Kv4Plan {
   int waves, splits;
 };
 Kv4Plan kv4_plan(int B, int Hkv, long max_len) {
   const long pairs = (long)B * Hkv, rounds = (max_len + KV4_WAVES * KV4_TILE - 1) / (KV4_WAVES * KV4_TILE);
-  long s = (1024 + pairs - 1) / pairs;
-  if (s > rounds) s = rounds;
-  if (s > 1 && pairs <= 256 && max_len <= (pairs > 64 ? 16 * pairs : 1024)) return {KV4_WIDE, 1};
-  return {KV4_WAVES, (int)(s < 1 ? 1 : s > 256 ? 256 : s)};
+  if (pairs > 256) return {KV4_WAVES, max_len <= 2048 ? 1 : (int)((1024 + pairs - 1) / pairs)};
+  if (max_len <= (pairs > 51 ? 20 * pairs : 1024)) return {KV4_WIDE, 1};
+  const long s = (B == 1 || max_len <= 8192 ? 512 : 1024) / pairs;
+  return {KV4_WAVES, (int)(s > rounds ? rounds : s > 256 ? 256 : s)};
 }
 
 }  // namespace
