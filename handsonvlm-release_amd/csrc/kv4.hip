@@ -79,9 +79,11 @@ __device__ __forceinline__ float quarter_sum(float v) {
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 constexpr int KV4_RING = 4;                // tiles in a wave's LDS ring
 
+// vmcnt(V), and lgkmcnt(0): the wave's reads of LDS are back too, so a slot that they read may be filled again
 template <int V>
-__device__ __forceinline__ void kv4_wait() {                                  // vmcnt(V)
-  __builtin_amdgcn_s_waitcnt((V & 15) | ((V >> 4) << 14) | 0xF70);
+__device__ __forceinline__ void kv4_wait() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((V & 15) | ((V >> 4) << 14) | 0x070);
   asm volatile("" ::: "memory");
 }
 
@@ -226,7 +228,7 @@ __device__ __forceinline__ void attn_decode_kv4_body(const Kv4Args& p) {
       // tile n has landed when no more than the tiles behind it are out
       const int behind = min(tiles - 1 - n, KV4_RING - 2);
       if (behind == 2) kv4_wait<2 * LOADS>(); else if (behind == 1) kv4_wait<LOADS>(); else kv4_wait<0>();
-      if (n + KV4_RING - 1 < tiles) fetch(n + KV4_RING - 1, (u + KV4_RING - 1) % KV4_RING);     // its slot's last reads fed products that are done with them
+      if (n + KV4_RING - 1 < tiles) fetch(n + KV4_RING - 1, (u + KV4_RING - 1) % KV4_RING);     // (tile n - 1's slot, whose reads the wait has seen back)
       compute(n, u);
     }
   }

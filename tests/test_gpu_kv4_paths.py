@@ -1,0 +1,45 @@
+"""Single-token attention over the 4-bit cache in every launch shape that it chooses between, against the definition in 64 bits: rings of tiles that
+wrap, splits of several rounds, more than 256 (sample, KV head) pairs on either side of 2048 keys."""
+import pytest
+import torch
+
+from test_gpu_mxfp4 import check_attn, gen, make_cache, ops  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+# A wave takes 32 keys at a time and holds four such tiles in its ring: the lengths end its first wave's work behind 1, 3, 4, 5, 8 and 9 tiles.
+PATHS = [  # B, H, Hkv, dh, max_len, lens, splits
+    # 288 pairs, up to 2048 keys: four waves a head, no split
+    (9, 32, 32, 128, 1200, [1200, 512, 513, 1024, 1025, 384, 385, 1, 0], 1),
+    (9, 32, 32, 64, 1200, [0, 33, 511, 512, 640, 1023, 1152, 1153, 1200], 1),
+    (5, 64, 64, 128, 700, [700, 513, 512, 31, 128], 1),
+    # beyond 2048 keys: 4 and 2 splits of several rounds
+    (9, 32, 32, 128, 4700, [4700, 2049, 2048, 513, 4096, 4097, 1, 0, 3000], 4),
+    (9, 32, 32, 64, 4700, [100, 4608, 4609, 2304, 0, 1024, 4700, 2500, 5], 4),
+    (16, 64, 32, 128, 2300, [2300, 2299, 2048, 2049, 1024, 1025, 0, 1, 512, 513, 128, 129, 700, 1800, 2177, 2176], 2),
+    # 128 pairs, one workgroup of eight waves a head, up to ten tiles a wave
+    (4, 32, 32, 128, 2500, [2500, 1280, 1281, 2304], 1),
+    (4, 32, 32, 64, 2500, [2305, 2500, 1024, 1025], 1),
+    # 64 pairs with shared heads and long caches: 16 splits of up to ten rounds
+    (8, 32, 8, 128, 20000, [20000, 8192, 8193, 16384, 1, 0, 10241, 19999], 16),
+    (8, 32, 8, 64, 20000, [16385, 20000, 4096, 129, 10240, 0, 18432, 7], 16),
+    # one sample, 32 heads, 16 splits
+    (1, 32, 32, 128, 12000, [11999], 16),
+    # 12 and 16 heads on one KV head
+    (2, 24, 2, 128, 1500, [1500, 1281], 12),
+    (2, 32, 2, 64, 1500, [1407, 1500], 12),
+]
+
+
+@pytest.mark.parametrize("B,H,Hkv,dh,n,lens,splits", PATHS)
+def test_attention_launch_shapes(ops, B, H, Hkv, dh, n, lens, splits):  # noqa: F811
+    from hvlm import _lib
+    assert _lib.load().hvlm_attn_decode_kv4_ws_bytes(B, H, Hkv, dh, n) == (0 if splits == 1 else B * H * splits * (dh + 2) * 4)
+    g = gen(B * 101 + H * 11 + n + dh)
+    cache = make_cache(ops, B, Hkv, n, dh, g)
+    q = torch.randn(B, H * dh, device="cuda", generator=g).to(BF16)
+    out = check_attn(ops, q, cache, torch.tensor(lens, dtype=torch.int32, device="cuda"), H, dh ** -0.5)
+    for b, m in enumerate(lens):
+        assert (out[b] == 0).all() == (m == 0)
