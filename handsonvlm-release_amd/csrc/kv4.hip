@@ -262,7 +262,7 @@ __device__ __forceinline__ void attn_decode_kv4_body(const Kv4Args& p) {
     }
     const long head = (long)b * p.H + hk * p.G + h;
     if (p.splits == 1) {
-      p.out[(long)b * p.ldo + (hk * p.G + h) * DH + d] = f2bf(den == 0.f ? 0.f : acc / den);
+      p.out[(long)b * p.ldo + (hk * p.G + h) * DH + d] = f2bf(len == 0 ? 0.f : acc / den);     // (keys whose scores are all -inf: 0 / 0, as the definition has it)
     } else {
       float* rec = p.ws + (head * p.splits + split) * (DH + 2);
       rec[d] = acc;
@@ -280,7 +280,8 @@ __global__ __launch_bounds__(KV4_WIDE * 64, 2) void attn_decode_kv4_64_wide_kern
 // in LDS, in order.
 constexpr int KV4_JOIN = 4;
 template <int DH>
-__global__ __launch_bounds__(KV4_JOIN * DH) void kv4_combine_kernel(const float* __restrict__ ws, bf16_t* __restrict__ out, long ldo, int H, int splits) {
+__global__ __launch_bounds__(KV4_JOIN * DH) void kv4_combine_kernel(const float* __restrict__ ws, const int32_t* __restrict__ lens, bf16_t* __restrict__ out, long ldo,
+                                                                   int H, int splits) {
   __shared__ float sa[KV4_JOIN][DH], sm[KV4_JOIN], sl[KV4_JOIN];
   const long head = blockIdx.x;
   const float* rec = ws + head * splits * (DH + 2);
@@ -324,7 +325,8 @@ __global__ __launch_bounds__(KV4_JOIN * DH) void kv4_combine_kernel(const float*
     acc += f * sa[i][d];
     den += f * sl[i];
   }
-  out[(head / H) * ldo + (head % H) * DH + d] = f2bf(den == 0.f ? 0.f : acc / den);
+  const long b = head / H;
+  out[b * ldo + (head % H) * DH + d] = f2bf(lens[b] <= 0 ? 0.f : acc / den);
 }
 
 // Splits of the key axis, waves of a workgroup, by the number of (sample, KV head) pairs and the length of the cache.  Two workgroups fit a CU.
@@ -409,6 +411,6 @@ extern "C" int hvlm_attn_decode_kv4(const void* q, long ldq, const void* k_codes
   const int rc2 = check_launch("attn_decode_kv4");
   if (rc2 || splits == 1) return rc2;
   const auto c = dh == 128 ? kv4_combine_kernel<128> : kv4_combine_kernel<64>;
-  hipLaunchKernelGGL(c, dim3((unsigned)(B * H)), dim3(KV4_JOIN * dh), 0, as_stream(stream), (const float*)ws, (bf16_t*)out, ldo, H, splits);
+  hipLaunchKernelGGL(c, dim3((unsigned)(B * H)), dim3(KV4_JOIN * dh), 0, as_stream(stream), (const float*)ws, lens, (bf16_t*)out, ldo, H, splits);
   return check_launch("attn_decode_kv4");
 }

@@ -43,3 +43,28 @@ def test_attention_launch_shapes(ops, B, H, Hkv, dh, n, lens, splits):  # noqa: 
     out = check_attn(ops, q, cache, torch.tensor(lens, dtype=torch.int32, device="cuda"), H, dh ** -0.5)
     for b, m in enumerate(lens):
         assert (out[b] == 0).all() == (m == 0)
+
+
+@pytest.mark.parametrize("B,H,Hkv,dh,n", [(2, 4, 2, 128, 300), (9, 32, 32, 64, 700), (2, 8, 8, 128, 3000)])
+def test_scores_that_are_not_finite(ops, B, H, Hkv, dh, n):  # noqa: F811
+    """What softmax makes of them: a head whose scores are all -inf has no result (0 / 0), no more than one with +inf or NaN among its scores.  The
+    other heads and samples keep their bits, and no keys still give zeros."""
+    g = gen(n)
+    cache = make_cache(ops, B, Hkv, n, dh, g)
+    G = H // Hkv
+    lens = torch.tensor([n, n - 37][:B] + [0] * (B - 2), dtype=torch.int32, device="cuda")
+    q = torch.randn(B, H * dh, device="cuda", generator=g).to(BF16)
+    want = check_attn(ops, q, cache, lens, H, dh ** -0.5)
+    h0 = G                                                                     # a query head on KV head 1, whose element 3 gets one sign in every key
+    nan = torch.zeros_like(want, dtype=torch.bool)
+    for code, bad in ((0x9, float("inf")), (0x2, float("-inf")), (0x2, float("inf")), (0x2, float("nan"))):
+        c, x = ops.KV4Cache(*(t.clone() for t in cache)), q.clone()
+        c.k[0, 1, :, 1] = (c.k[0, 1, :, 1] & 0x0F) | (code << 4)              # -0.5 or 1
+        x[0, h0 * dh + 3] = bad
+        got = ops.attn_decode_kv4(x, c, lens, H, dh ** -0.5)
+        nan[:] = False
+        nan[0, h0 * dh:(h0 + 1) * dh] = True
+        assert torch.equal(torch.isnan(got), nan), (code, bad)
+        keep = ~nan
+        keep[0, G * dh:2 * G * dh] = False                                     # (KV head 1's other heads see other keys)
+        assert torch.equal(got[keep], want[keep])
