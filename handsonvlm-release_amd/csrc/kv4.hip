@@ -14,8 +14,10 @@
 // The codes of a tile (K 2 KB, V 2 KB) come by LDS-DMA, 1 KB of consecutive rows an instruction, into a ring of the wave's own, three tiles ahead
 // and without a barrier; loaded into registers in fragment order a tile would take 20 instructions instead of 6 and the address units
 // would bound the kernel.  A tile's scales are two more.
-// Softmax: running maximum and sum per wave in fp32; P is rounded to bf16 for the second product (its error, at most 2^-8 relative and
-// independent from key to key, is below that of the bf16 result).  The waves of a workgroup take alternate tiles and merge in LDS; the
+// Softmax: running maximum and sum per wave in fp32.  P enters the second product as two bf16 terms, its rounding and the rounded rest, 2^-16 relative
+// in all: with the first alone keys of equal scores would all be off by the same up to 2^-8, as much as the result's own rounding.  Up to eight heads
+// leave half of the sixteen columns free: column r + 8 repeats head r and carries the rests, so that the second term costs no product; nine to sixteen
+// heads have it in products of its own.  The waves of a workgroup take alternate tiles and merge in LDS; the
 // workgroups of a split sample write (max, sum, unnormalised row) in fp32 and a second kernel joins them in order: no atomics.
 // Rows at and past lens[b] are never read.
 //
@@ -76,6 +78,10 @@ __device__ __forceinline__ float quarter_sum(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
+__device__ __forceinline__ float kv4_other_half(float v) {                    // of the lane eight columns away
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xF, 0xF, true));     // row_ror:8
+}
+
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 constexpr int KV4_RING = 4;                // tiles in a wave's LDS ring
 
@@ -112,6 +118,7 @@ __device__ __forceinline__ void attn_decode_kv4_body(const Kv4Args& p) {
 #pragma unroll
   for (int j = 0; j < VD; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
   float mx = -INFINITY, sum = 0.f;
+  const bool second = p.G <= 8 && r16 >= 8;                                    // a column of the second terms
 
   char* const ring = reinterpret_cast<char*>(sm) + w * (KV4_RING * SLOT);
   const int krow = 4 * (r16 & 3) + (r16 >> 2);
@@ -185,7 +192,13 @@ __device__ __forceinline__ void attn_decode_kv4_body(const Kv4Args& p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) { pr[e] = __builtin_amdgcn_exp2f(s[e] - off); ps += pr[e]; }
     sum = sum * fac + ps;                                                      // (this lane's quarter of the keys; joined at the end)
-    const u32x4 pw = {pack_bf2(pr[0], pr[1]), pack_bf2(pr[2], pr[3]), pack_bf2(pr[4], pr[5]), pack_bf2(pr[6], pr[7])};
+    u32x4 pw, rest;                                                            // two probabilities a dword; p less its rounding
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned h = pack_bf2(pr[2 * i], pr[2 * i + 1]);
+      rest[i] = pack_bf2(pr[2 * i] - bf_lo(h), pr[2 * i + 1] - bf_hi(h));
+      pw[i] = second ? rest[i] : h;
+    }
     const bf16x8 pf = __builtin_bit_cast(bf16x8, pw);
 #pragma unroll
     for (int j = 0; j < VD; ++j) o[j] *= fac;
@@ -209,13 +222,15 @@ __device__ __forceinline__ void attn_decode_kv4_body(const Kv4Args& p) {
       for (int e = 0; e < 4; ++e)
         f[e] = __builtin_amdgcn_perm(vp[j >> 1][2 * e + 1], vp[j >> 1][2 * e], (j & 1) ? 0x07060302u : 0x05040100u);
       o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, f), pf, o[j], 0, 0, 0);
+      if (p.G > 8) o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, f), __builtin_bit_cast(bf16x8, rest), o[j], 0, 0, 0);
     }
   };
 #pragma unroll
   for (int n = 0; n < KV4_RING - 1; ++n)
     if (n < tiles) fetch(n, n);
   {
-    const bf16_t* qp = p.q + (long)b * p.ldq + (long)(hk * p.G + min(r16, p.G - 1)) * DH + g * KD;   // (columns past G repeat the last head)
+    const int head = min(p.G > 8 ? r16 : r16 & 7, p.G - 1);                    // of this column (those past G repeat the last head)
+    const bf16_t* qp = p.q + (long)b * p.ldq + (long)(hk * p.G + head) * DH + g * KD;
 #pragma unroll
     for (int j = 0; j < KD / 8; ++j) qf[j] = *reinterpret_cast<const bf16x8*>(qp + j * 8);
   }
@@ -235,6 +250,12 @@ __device__ __forceinline__ void attn_decode_kv4_body(const Kv4Args& p) {
   sum = quarter_sum(sum);
   __syncthreads();                                                             // the rings become the rows to merge
 
+  if (p.G <= 8) {
+#pragma unroll
+    for (int j = 0; j < VD; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[j][i] += kv4_other_half(o[j][i]);
+  }
   // merge: lane holds dims (4 g + i) VD + j of head r16
   float* sm_m = sm + WAVES * p.G * DH;
   float* sm_l = sm_m + WAVES * p.G;

@@ -1,9 +1,11 @@
 """Single-token attention over the 4-bit cache in every launch shape that it chooses between, against the definition in 64 bits: rings of tiles that
 wrap, splits of several rounds, more than 256 (sample, KV head) pairs on either side of 2048 keys."""
+import math
+
 import pytest
 import torch
 
-from test_gpu_mxfp4 import check_attn, gen, make_cache, ops  # noqa: F401
+from test_gpu_mxfp4 import HALF_STEP, attn_ref, check_attn, gen, make_cache, ops  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
@@ -68,3 +70,36 @@ def test_scores_that_are_not_finite(ops, B, H, Hkv, dh, n):  # noqa: F811
         keep = ~nan
         keep[0, G * dh:2 * G * dh] = False                                     # (KV head 1's other heads see other keys)
         assert torch.equal(got[keep], want[keep])
+
+
+PRECISE = [(1, 32, 32, 128, 967, [967]), (9, 32, 32, 64, 700, [700, 513, 31] * 3), (2, 8, 1, 128, 3000, [3000, 1111]), (2, 18, 2, 128, 500, [500, 77]),
+           (2, 16, 1, 64, 1500, [1500, 1281]), (9, 64, 32, 128, 2500, [2500, 2049, 1000] * 3)]
+
+
+@pytest.mark.parametrize("B,H,Hkv,dh,n,lens", PRECISE)
+def test_equal_scores_leave_a_constant_value_as_it_is(ops, B, H, Hkv, dh, n, lens):  # noqa: F811
+    """Every value row is 1, so every result is 1.  One key in 32 scores 0.6916.. above the others, whose probability 0.5 (1 + 2^-8 - 2^-12) lies
+    just short of half a bf16 step above 0.5: rounded there and not in their sum, they would lose 2^-8 of it together.  What 32 bits lose, (n + 8) 2^-23, and what two bf16 terms lose,
+    2^-16, is far from half a step below 1, which is 2^-9."""
+    cache = ops.KV4Cache(*(torch.full(t.shape, fill, dtype=torch.uint8, device="cuda")
+                           for t, fill in zip(ops.KV4Cache.empty(B, n, Hkv, dh, "cuda"), (0x00, 127, 0x22, 127))))
+    cache.k[..., 0] = 0x01                                                     # 0.5 in element 0,
+    cache.k[:, :, ::32, 0] = 0x02                                              # 1 in every 32nd row
+    q = torch.zeros(B, H, dh, dtype=BF16, device="cuda")
+    q[:, :, 0] = 1.0
+    scale = -2.0 * math.log(0.5 * (1 + 2.0 ** -8 - 2.0 ** -12))
+    out = ops.attn_decode_kv4(q.view(B, H * dh), cache, torch.tensor(lens, dtype=torch.int32, device="cuda"), H, scale)
+    assert (out == 1).all(), out.unique()
+
+
+@pytest.mark.parametrize("B,H,Hkv,dh,n,lens", PRECISE)
+def test_probabilities_are_not_rounded_to_bf16(ops, B, H, Hkv, dh, n, lens):  # noqa: F811
+    """The bound of test_attention_shapes with 2^-16 of p |v| for the two terms of P in the place of 2^-8 for a single one."""
+    g = gen(B + H + n)
+    cache = make_cache(ops, B, Hkv, n, dh, g)
+    q = torch.randn(B, H * dh, device="cuda", generator=g).to(BF16)
+    got = ops.attn_decode_kv4(q, cache, torch.tensor(lens, dtype=torch.int32, device="cuda"), H, dh ** -0.5)
+    want, tol = attn_ref(q, cache, lens, H, dh ** -0.5)
+    mean, _ = attn_ref(q, cache._replace(v=cache.v & 0x77), lens, H, dh ** -0.5)           # p |v|: codes without their signs
+    tol = tol - (HALF_STEP - 2.0 ** -16) * mean
+    assert ((got.double() - want).abs() <= tol).all()
