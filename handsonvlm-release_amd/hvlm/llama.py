@@ -393,16 +393,23 @@ class LlamaStack:
             self.__dict__.pop("_dec_graphs_b", None)        # a captured decode step points at the old copies
             self._mxfp4_w = [{k: ops.quantize_mxfp4(lp.w[k]) for k in ("qkv", "o", "gu", "down")} for lp in self.layers]
 
-    def _mm_mxfp4(self, li: int, key: str, a: torch.Tensor, residual=None) -> torch.Tensor:
+    def _mm_mxfp4(self, li: int, key: str, a: torch.Tensor, residual=None, decode: bool = False) -> torch.Tensor:
+        """Prefill: activations in 4 bits as well.  Decode steps: bf16 activations, 32 rows per read of the weights (the cost is that read).  The number of
+        rows decides nothing, so that a sample's arithmetic does not depend on its batch."""
         w4 = self._mxfp4_w[li][key]
-        if a.shape[0] <= 32:        # decode steps: the cost is reading W once, the activations stay bf16 (no rounding of them)
+        if not decode:
+            return ops.gemm_mxfp4_nt(ops.quantize_mxfp4(a), w4, residual=residual)
+        if a.shape[0] <= 32:
             return ops.gemm_w4a16_nt(a, w4, residual=residual)
-        return ops.gemm_mxfp4_nt(ops.quantize_mxfp4(a), w4, residual=residual)
+        out = torch.empty((a.shape[0], w4[0].shape[0]), dtype=BF16, device=a.device)
+        for r in range(0, a.shape[0], 32):
+            ops.gemm_w4a16_nt(a[r:r + 32], w4, residual=None if residual is None else residual[r:r + 32], out=out[r:r + 32])
+        return out
 
-    def _layer_mm(self, li: int, fp8: bool, mxfp4: bool):
+    def _layer_mm(self, li: int, fp8: bool, mxfp4: bool, decode: bool = False):
         """mm(a, key, residual) = a @ W_key^T (+ residual) of layer li in the weight format asked for."""
         if mxfp4:
-            return lambda a, k, residual=None: self._mm_mxfp4(li, k, a, residual)
+            return lambda a, k, residual=None: self._mm_mxfp4(li, k, a, residual, decode)
         if fp8:
             return lambda a, k, residual=None: self._mm_fp8(li, k, a, residual)
         w = self.layers[li].w
@@ -479,7 +486,7 @@ class LlamaStack:
         fused = (_DECODE_FUSED_FINALIZE and ops._GEMM_SKINNY and x1.is_cuda and B <= 32 and self.D % 64 == 0 and self.F % 4 == 0
                  and self.D >= 256 and self.dh % 8 == 0 and not mxfp4)
         for li, lp in enumerate(self.layers):
-            mm = self._layer_mm(li, fp8, mxfp4)
+            mm = self._layer_mm(li, fp8, mxfp4, decode=True)
             wsel = (lambda k: self._fp8_rw[li][k]) if fp8 else (lambda k: lp.w[k])
             xn, _ = ops.rmsnorm_fwd(x, lp.w["ln1"], eps, save_rstd=False)
             if fused and not kv4:
