@@ -165,14 +165,15 @@ class LlamaStack:
     def new_cache(self, max_len: Optional[int] = None, batch: Optional[int] = None, kv4: bool = False) -> list:
         """Per-layer [max_len, 3D] buffers in the fused qkv layout (k at column D, v at 2D); with `batch`: [B, max_len, 3D]
         (lock-step generation of B samples).  kv4 (with `batch`): one ops.KV4Cache per layer instead, keys and values in MXFP4 —
-        1.06 bytes per position and feature of D against the 6 of the bf16 buffer (which holds q's columns too)."""
+        1.06 bytes per position and feature of D against the 6 of the bf16 buffer (which holds q's columns too).  One batched cache is
+        kept for the next call; asking for the other format lets it go."""
         n = max_len or self.cfg.max_position_embeddings
         if kv4:
             assert batch is not None, "the 4-bit cache belongs to the lock-step decode (batch=...)"
             kept = getattr(self, "_kv4_cache_b", None)
             if kept is None or kept[0].k.shape[0] != batch or kept[0].k.shape[2] < n:
                 kept = None
-                self._kv4_cache_b = None                    # (as below: the old cache and the graphs captured on it go first)
+                self._kv4_cache_b = self._kv_cache_b = None     # (as below: the old cache, of either format, and the graphs captured on it go first)
                 self.__dict__.pop("_dec_graphs_b", None)
                 kept = [ops.KV4Cache.empty(batch, n, self.H, self.dh, self.device) for _ in range(self.L)]
                 self._kv4_cache_b = kept
@@ -181,7 +182,7 @@ class LlamaStack:
             kept = getattr(self, "_kv_cache_b", None)
             if kept is None or kept[0].shape[0] != batch or kept[0].shape[1] < n:
                 kept = None
-                self._kv_cache_b = None                     # free the old one before allocating (22 GB at B = 32)
+                self._kv_cache_b = self._kv4_cache_b = None     # free the old one before allocating (22 GB at B = 32)
                 self.__dict__.pop("_dec_graphs_b", None)    # (and the decode graph captured on it)
                 kept = [torch.empty((batch, n, 3 * self.D), dtype=BF16, device=self.device) for _ in range(self.L)]
                 self._kv_cache_b = kept

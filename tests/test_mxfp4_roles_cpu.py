@@ -58,3 +58,20 @@ def test_prefill_quantises_its_activations(monkeypatch, B, S):
     assert calls == ["quantize", "gemm"] * (4 * st.L)
     alone = st.forward(x, 1, S, save=False, mxfp4=True).double().repeat(B, 1)
     assert (got - alone).norm() <= (9 * st.L + 1) * 2.0 ** -8 * alone.norm()
+
+
+def test_one_batched_cache_is_kept(monkeypatch):
+    """The cache of the other format, and what was captured on it, does not stay beside the new one."""
+    import gc
+    import weakref
+    installed(monkeypatch)
+    st = _model().stack
+    for first in (False, True, False):
+        cache = st.new_cache(8, batch=2, kv4=first)
+        assert st.new_cache(6, batch=2, kv4=first) is cache
+        st._dec_graphs_b = {"captured": cache}
+        seen = [weakref.ref(t) for layer in cache for t in (layer if first else [layer])]
+        del cache
+        st.new_cache(8, batch=2, kv4=not first)
+        gc.collect()
+        assert "_dec_graphs_b" not in st.__dict__ and not any(r() is not None for r in seen)
