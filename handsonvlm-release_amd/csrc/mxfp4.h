@@ -3,7 +3,8 @@
 // nibble.  A block is quantised with s - 127 = floor(log2 max|x|) - 2 (6 = 1.5 * 2^2 is the largest element: values between 6 and 8 of a
 // block saturate, as the format's specification has it) and round-to-nearest-even; a block with an infinity or a NaN becomes NaN.
 // v_cvt_scalef32_pk_* does the scaling and the rounding of a pair in one instruction; it agrees with the definition for every finite
-// bf16 / fp16 value at every scale code, and for every code back to bf16 / fp16 / fp32, subnormal results included.
+// bf16 / fp16 value at every scale code, and for every code back to bf16 / fp16 / fp32, subnormal results included (4 and 6 at scale code 253, 2 and
+// more at 254 are past the range of bf16 and fp32 and become infinities; no quantised block has a scale code above 252).
 #pragma once
 #include "common.h"
 
@@ -58,7 +59,7 @@ __device__ __forceinline__ unsigned mx_quant8(u32x4 v, unsigned s) {
   }
   return s == 255u ? 0u : r;                         // a NaN block holds zeros under its NaN scale
 }
-// byte I of a dword of codes -> a bf16 pair (exact)
+// byte I of a dword of codes -> a bf16 pair (exact but for overflow)
 template <int I>
 __device__ __forceinline__ unsigned mx_pair_bf16(unsigned codes, float sc) {
   return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, sc, I));

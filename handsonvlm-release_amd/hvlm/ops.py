@@ -423,7 +423,7 @@ def quantize_mxfp4(x: torch.Tensor, out=None):
 
 
 def dequantize_mxfp4(q, out_dtype=BF16) -> torch.Tensor:
-    """(codes, scales) -> [R, K] values in bf16 (exact) or fp16."""
+    """(codes, scales) -> [R, K] values in bf16 (exact; past its range, which starts at 2^128, infinities) or fp16."""
     codes, scales, R, K, ldc, lds = _mx_pair("dequantize_mxfp4", q)
     if out_dtype != BF16 and out_dtype != F16:
         _fail(f"dequantize_mxfp4: bf16 or fp16, not {out_dtype}")

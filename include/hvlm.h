@@ -496,7 +496,8 @@ int hvlm_cast_bf16_to_f32(const void* in, float* out, long n, void* stream);
  * its own to match, parity = the definition below in 64 bits.
  *   codes  : 4-bit E2M1 {0, 0.5, 1, 1.5, 2, 3, 4, 6} with a sign bit, two per byte, the even element in the low nibble: K / 2 bytes a row
  *   scales : one E8M0 byte s per 32 elements, 2^(s - 127); 255 = the whole block is NaN: K / 32 bytes a row, at any alignment
- *   value  : code * 2^(s - 127)
+ *   value  : code * 2^(s - 127).  What lies past the range of bf16 (and of fp32) - 4 and 6 at s = 253, 2 and more at s = 254 - is an infinity wherever values are
+ *            taken to bf16: in dequantize, as a weight of gemm_w4a16, as a key or value of the attention.  quantize makes no scale above 252.
  * Leading dimensions of codes and scales are in BYTES.  Every K is a multiple of 32.  Outputs overlap no input, but where noted.
  * ------------------------------------------------------------------------------------------ */
 /* x [rows, K] (bf16, or IEEE half when f16 != 0; ldx elements) -> codes, scales: s - 127 = floor(log2(max |x|)) - 2 (at least -127),
@@ -504,7 +505,7 @@ int hvlm_cast_bf16_to_f32(const void* in, float* out, long n, void* stream);
  * rows of codes 4-byte aligned; rows * K / 8 < 2^31. */
 int hvlm_quantize_mxfp4(const void* x, void* codes, void* scales, int rows, int K, long ldx, long ld_codes, long ld_scales, int f16,
                         void* stream);
-/* The values back as bf16 (exact) or IEEE half (f16 != 0; rounds, overflows to infinity). */
+/* The values back as bf16 (exact within its range) or IEEE half (f16 != 0; rounds, overflows to infinity). */
 int hvlm_dequantize_mxfp4(const void* codes, const void* scales, void* out, int rows, int K, long ld_codes, long ld_scales, long ldo,
                           int f16, void* stream);
 /* C[M, N] = act(A[M, K] @ B[N, K]^T + bias[N]) + residual[M, N], both operands MXFP4, fp32 accumulation on the scaled MFMA.  C is bf16, or
