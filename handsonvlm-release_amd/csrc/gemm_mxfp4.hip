@@ -12,12 +12,14 @@
 //     step is 64 products without a wait, with the next step's 17 LDS reads and 8 LDS-DMA pieces strewn between them one at a time;
 //   * codes go from global memory to LDS by DMA in rows of 128 bytes (rows of 64 halve the L2's rate: 16.7 instead of 32 TB/s), addressed by a
 //     register that runs along, with 16-byte chunks permuted by c ^ (row & 7): eight rows of a fragment read fall into eight bank groups;
-//   * scales are tiled once per call by a kernel of their own (3 us at 22 016 rows of 4096) so that a step's fit one dword per four fragments:
+//   * scales are tiled once per call by a kernel of their own (3.6 us for 867 + 12 288 rows of 4096, 5.3 for 13 872 + 22 016) so that a step's fit one dword per four fragments:
 //     gathered row by row inside the K loop they cost a quarter of it (0.15 of 0.78 us a step);
 //   * workgroups are persistent and the ring runs on into the next tile, whose first 512 k land during the last of this one.
-// 13872 x 22016 x 4096: 579 us = 4.3 PFLOP/s (two groups of four waves one barrier apart, the shape of gemm_pp.hip: 723 us).  Without DMA and
-// scales a step would take 0.46 us instead of 0.62, the products alone 0.43; the rest is the tiles' ends (vision shapes with K = 1024 are
-// mostly that: 90 us where the result's bytes need 44).
+// 13872 x 22016 x 4096: median 646 us = 3.9 PFLOP/s over inputs that change from call to call (the best of such runs 579 - 612; two groups of four
+// waves one barrier apart, the shape of gemm_pp.hip, 723 at best).  Without DMA and scales a step would take 0.46 us instead of 0.62, the products alone 0.43; the
+// rest is the tiles' ends (vision shapes with K = 1024 are mostly that: 90 us where the result's bytes need 44).
+// Registers: the 256 x 256 kernel keeps 132 scalars in lanes of vector registers (the 128 x 128 one 55), tile coordinates and the epilogue's addresses; they are
+// saved and fetched between tiles, the body of the K loop touches none of them.
 #include "mxfp4.h"
 #include <algorithm>
 #include <type_traits>

@@ -9,8 +9,8 @@
 // workgroup and slice in LDS.  K-slices are summed, in order, from fp32 slabs by a second small kernel with the epilogue; with one to four rows
 // of x the slices are the waves of one workgroup and no second kernel runs.
 //
-// Bound by the read of W where W is large: 22016 x 4096 at one row 11.2 us (4.3 TB/s; a copy's rate would take 10.0 us),
-// 32101 x 4096 at 32 rows 21.9 us + 4.8 us to sum the slabs (15.1 us; there the staging of x, as many bytes from L2 as W has, and the slabs, 16 MB, come on top).
+// Bound by the read of W where W is large: 22016 x 4096 at one row 10.8 us (4.4 TB/s; a copy's rate would take 10.0 us),
+// 32101 x 4096 at 32 rows 21.2 us + 4.6 us to sum the slabs (15.1 us; there the staging of x, as many bytes from L2 as W has, and the slabs, 16 MB, come on top).
 #include "mxfp4.h"
 
 namespace hvlm {

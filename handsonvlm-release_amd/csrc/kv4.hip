@@ -21,9 +21,10 @@
 // workgroups of a split sample write (max, sum, unnormalised row) in fp32 and a second kernel joins them in order: no atomics.
 // Rows at and past lens[b] are never read.
 //
-// Bound by the read of the cache when there are many keys: 32 samples x 32 heads, 98 MB, 28 - 30 us; 8 samples x 8 KV
-// heads of up to 32768 keys, 214 MB, 40 - 49 us and 4.7 us to join (from HBM at the rate of a copy, 4.79 TB/s, these take 20 and 45 us; what earlier
-// calls left in the last-level cache comes faster).  Short caches by latency: one sample x 32 heads x 1024 keys 9 us.
+// Bound by the read of the cache when there are many keys: 32 samples x 32 heads, 98 MB, 32 - 34 us; 8 samples x 8 KV
+// heads of up to 32768 keys, 214 MB, 52 us and 4.6 us to join (from HBM at the rate of a copy, 4.79 TB/s, these take 20 and 45 us; what earlier
+// calls left in the last-level cache comes faster).  Short caches by latency: one sample x 32 heads x 967 keys 9.6 us.  (Medians.  The second term of P is 0.1 to
+// 0.9 us of each, or 5 % at most.)
 #include "mxfp4.h"
 
 namespace hvlm {
@@ -354,9 +355,10 @@ __global__ __launch_bounds__(KV4_JOIN * DH) void kv4_combine_kernel(const float*
 //   Up to 256 pairs, short caches: a workgroup of eight waves reads all of a head's keys and nothing is joined.  Longer ones: one round of splits (512
 //   workgroups), joined by a second kernel; where samples may differ by many thousands of keys two rounds, so that the short ones make room.
 //   Beyond 256 pairs: no split, but for long caches, whose last round would be long.
-// Measured (us; all keys used, dh = 128): 32 pairs x 256 keys one kernel 4.9, two 6.4; x 1024 9.1 / 8.1 (and a launch of the host more);
-// x 8192 8, 16, 32 splits 16.2, 16.7, 20.1; 128 pairs x 2048 one kernel 16.1, two 15.6, x 4096 26.0 / 21.5; 64 pairs x 32768 8, 16 splits 60.6, 64.4, but 49 / 41
-// with lengths spread from 1000 to 32768; 520 pairs x 967 1, 2 splits 24.1, 26.5, x 4096 75.5, 68.2.
+// Measured (us, in a graph; all keys used, dh = 128): 32 pairs x 256 keys one kernel 5.5, two 7.2; x 512 7.0 / 7.5; x 967 9.6 / 8.2: from about 600 keys on the
+// second launch costs a graph less than it gains, but a call that is issued by itself some 3 us of the host.  x 8192 8, 16, 32 splits 17.0, 16.9, 20.0;
+// 128 pairs x 2048 one kernel 16.9, two 16.2, x 4096 28.0 / 22.8; 64 pairs x 32768 8, 16 splits 68.7, 74.3, and 42.5, 42.6 with lengths spread from 1000 to
+// 32768; 520 pairs x 967 1, 2 splits 26.3, 27.8, x 4096 82.8, 74.9; 1024 pairs x 1131 38.5, 47.1.
 struct Kv4Plan {
   int waves, splits;
 };

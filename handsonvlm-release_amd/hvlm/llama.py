@@ -420,7 +420,7 @@ class LlamaStack:
         """One new token for each of B samples in lock step: x1 [B, D], lens int32 [B] (device) = position of the new token
         of every sample = its current cache length; cache[l] [B, max_len, 3D] or an ops.KV4Cache (new_cache(kv4=True)); the four
         projections in bf16, e4m3 (fp8) or MXFP4 (mxfp4) weights, in any combination with the cache.  Returns the final-normed hidden [B, D]
-        (valid until the next call).  Weights are streamed once per step for all B samples (GEMMs at M = B).
+        (valid until the next call).  Weights are streamed once per step for all B samples (GEMMs at M = B; MXFP4 weights once for every 32).
 
         The step is ~450 short launches (5 - 80 us each) and the generation loop needs its result on the host before it can
         issue the next one, so issuing them from Python is what bounds it once the kernels are fast (7.4 ms issued eagerly

@@ -776,7 +776,7 @@ class HandsOnVLMForCausalLM:
         batched prefill (bf16, or the e4m3 GEMMs with `fp8`) filling a [B, max_len, 3D] KV cache per layer and one batched
         decode step per generated token (weights streamed once for all B samples; e4m3 weights with `fp8_decode`).
         `fp8_clip` runs the CLIP tower's layer GEMMs on e4m3 operands as well.  `mxfp4` / `mxfp4_decode`: the same two places in
-        MXFP4 (4-bit weights and activations in the prefill, 4-bit weights in the decode steps); `kv4`: keys and values are kept in
+        MXFP4 (4-bit weights and activations in the prefill, 4-bit weights and bf16 activations in the decode steps, whatever the batch); `kv4`: keys and values are kept in
         MXFP4 (a quarter of their bytes; the prefill itself attends to the unrounded ones).  Right-padded prompts (attention_mask)
         are supported: a sample's pad rows are never attended (its own length bounds its keys).
         `logits_processor`: callables (input_ids [B, cur], scores [B, V]) -> scores.  `hand_noise[b][j]`: optional z for the

@@ -525,7 +525,8 @@ int hvlm_gemm_w4a16_nt(const void* x, const void* W, const void* w_scale, void* 
  *   append: row (b, s) of qkv [B * S, ld] (q | k | v columns: H, Hkv and Hkv heads; k after RoPE) -> cache row start[b] + s of sample b.
  *       start (NULL: 0) and count (NULL: S; rows s >= count[b] are skipped) are device int32 [B]; rows outside the cache are dropped.
  *   attn_decode: out[b, h] = softmax(scale * q[b, h] . K)[t < lens[b]] V for one query row per sample; head h reads KV head
- *       h / (H / Hkv), H / Hkv <= 16.  lens: device int32 [B], clamped to 0 .. max_len; a sample of length 0 gives zeros.  Cache rows at and
+ *       h / (H / Hkv), H / Hkv <= 16.  lens: device int32 [B], clamped to 0 .. max_len; a sample of length 0 gives zeros, scores that are all -inf or hold
+ *       +inf or NaN give NaN, and so does an infinity among the values.  Probabilities are held to 2^-16.  Cache rows at and
  *       past lens[b] are never read.  ws: as above, hvlm_attn_decode_kv4_ws_bytes() bytes (0: may be NULL). */
 int hvlm_kv4_append(const void* qkv, long ld, void* k_codes, void* k_scales, void* v_codes, void* v_scales, const int32_t* start,
                     const int32_t* count, int B, int S, long max_len, int H, int Hkv, int dh, void* stream);
