@@ -23,8 +23,8 @@
 //
 // Bound by the read of the cache when there are many keys: 32 samples x 32 heads, 98 MB, 32 - 34 us; 8 samples x 8 KV
 // heads of up to 32768 keys, 214 MB, 52 us and 4.6 us to join (from HBM at the rate of a copy, 4.79 TB/s, these take 20 and 45 us; what earlier
-// calls left in the last-level cache comes faster).  Short caches by latency: one sample x 32 heads x 967 keys 9.6 us.  (Medians.  The second term of P is 0.1 to
-// 0.9 us of each, or 5 % at most.)
+// calls left in the last-level cache comes faster).  Short caches by latency: one sample x 32 heads x 967 keys 9.6 us.  (Medians.  Of these the second term of P is
+// 0.5 to 1.7 us, 5 % at most.)
 #include "mxfp4.h"
 
 namespace hvlm {

@@ -103,3 +103,44 @@ def test_probabilities_are_not_rounded_to_bf16(ops, B, H, Hkv, dh, n, lens):  # 
     mean, _ = attn_ref(q, cache._replace(v=cache.v & 0x77), lens, H, dh ** -0.5)           # p |v|: codes without their signs
     tol = tol - (HALF_STEP - 2.0 ** -16) * mean
     assert ((got.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("B,H,Hkv,dh,n", [(9, 32, 32, 128, 700), (9, 32, 32, 64, 4700), (4, 32, 32, 128, 2500), (2, 24, 2, 128, 1500), (8, 32, 8, 128, 20000)])
+def test_streams_and_graphs_at_once(ops, B, H, Hkv, dh, n):  # noqa: F811
+    """Append and attention of two caches on two streams at once, then from two graphs replayed with eager work between: the bits of one call by itself."""
+    g = gen(B + n)
+    caches = [make_cache(ops, B, Hkv, n, dh, g) for _ in range(2)]
+    qkv = [torch.randn(B, (H + 2 * Hkv) * dh, device="cuda", generator=g).to(BF16) for _ in range(2)]
+    lens = [torch.randint(0, n, (B,), device="cuda", generator=g).to(torch.int32) for _ in range(2)]
+    lens1 = [t + 1 for t in lens]
+
+    def step(i):
+        ops.kv4_append(qkv[i], caches[i], lens[i], H)
+        return ops.attn_decode_kv4(qkv[i], caches[i], lens1[i], H, dh ** -0.5)
+
+    want = [step(0), step(1)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(i))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for i in range(2):
+        with torch.cuda.graph(graphs[i]):
+            outs.append(step(i))
+    for r in range(3):
+        for i in range(2):
+            qkv[i].copy_(torch.randn(qkv[i].shape, device="cuda", generator=g))
+            lens[i].copy_((lens[i] + 17 * r) % n)
+            lens1[i].copy_(lens[i] + 1)
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        first = [o.clone() for o in outs]
+        assert all(torch.equal(step(i), first[i]) for i in range(2))
