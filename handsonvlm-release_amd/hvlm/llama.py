@@ -462,7 +462,7 @@ class LlamaStack:
                     out = self._decode_step_batched_eager(sx, sl, cache, fp8, mxfp4)
             finally:
                 ops.set_gemm_hook(hook)
-            st = (g, sx, sl, out, cache if isinstance(cache[0], ops.KV4Cache) else None)     # (a 4-bit cache lives as long as its graph)
+            st = (g, sx, sl, out, cache)                # (a cache lives as long as its graph: its addresses are in the key)
             graphs[key] = st
         g, sx, sl, out, _ = st
         sx.copy_(x1)

@@ -38,3 +38,23 @@ def test_a_short_prompt_is_prefilled_as_in_a_batch(S):
     many = st.forward(x.repeat(40, 1), 40, S, save=False, mxfp4=True)
     for b in (0, 17, 39):
         near(many[b * S:(b + 1) * S], alone, tolerance(st))
+
+
+@pytest.mark.parametrize("kv4", [False, True])
+def test_a_cache_lives_as_long_as_the_graph_captured_on_it(kv4):
+    """A graph is found again by its cache's address, so the address is not given to another cache while the graph is there."""
+    import gc
+    import weakref
+    st = model().stack
+    cache = st.new_cache(24, batch=2, kv4=kv4)
+    other = st.new_cache(24, batch=2, kv4=not kv4)                                # lets go of the first one
+    x = torch.zeros(2, st.D, dtype=BF16, device=DEV)
+    st.decode_step_batched(x, torch.zeros(2, dtype=torch.int32, device=DEV), cache)
+    seen = [weakref.ref(t) for layer in cache for t in (layer if kv4 else [layer])]
+    del cache
+    gc.collect()
+    assert len(st._dec_graphs_b) == 1 and all(r() is not None for r in seen)
+    assert st.new_cache(24, batch=2, kv4=not kv4) is other and all(r() is not None for r in seen)
+    st.invalidate_fp8()
+    gc.collect()
+    assert all(r() is None for r in seen)
